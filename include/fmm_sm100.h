@@ -68,6 +68,9 @@ typedef struct CUstream_st* fmm_stream_t; /* == cudaStream_t */
 #define FMM_DTYPE_BF16 0
 #define FMM_DTYPE_F16 1
 #define FMM_DTYPE_BF16_BF16 2
+/* element type of a row operand only: the X of fmm_quantize_rows, the gain of
+ * fmm_rms_norm_int8 */
+#define FMM_DTYPE_F32 3
 
 /* fmm_linear flags */
 #define FMM_LINEAR_PREPACKED 1u /* `Rt` already holds the packed right planes; W is ignored */
@@ -218,6 +221,44 @@ int fmm_linear(int scheme, int dtype, const void* A, const void* W, const void* 
  * Python plans always allocate through PyTorch). */
 int fmm_linear_noalloc(int scheme, const void* A, const void* W, const void* bias, void* C,
                        int64_t M, int64_t K, int64_t N, fmm_stream_t stream);
+
+/* ---- 8-bit integer linear -------------------------------------------------
+ * Codes are symmetric 8-bit integers with one FP32 scale a row (a token of the
+ * activations, an output channel of the weight); the value of a code is
+ * code * scale.  Code rows that fmm_linear_int8 reads start on 16-byte
+ * boundaries (base and leading dimension); bytes between a row's end and the
+ * next row are neither read nor written.  No counterparts in the reference,
+ * which has no quantised operator.  Zero rows are a no-op. */
+
+/* X[rows,cols] (FMM_DTYPE_BF16, FMM_DTYPE_F16 or FMM_DTYPE_F32, ldx) ->
+ * codes[rows,cols] (ldq) and scales[rows]:
+ *   a = max_k |x_k|,  scale = a / 127,  code_k = round_half_even(127 x_k / a)
+ * with the codes of exact arithmetic.  A row of zeros has codes 0 and scale 0;
+ * a row with an infinity or a NaN has codes 0 and a NaN scale. */
+int fmm_quantize_rows(int dtype, const void* X, int64_t rows, int64_t cols, int64_t ldx, int8_t* codes,
+                      int64_t ldq, float* scales, fmm_stream_t stream);
+
+/* Root-mean-square norm with the residual's addition and an 8-bit output:
+ *   h = X + residual, rounded to dtype and stored to residual_out
+ *       (residual NULL: h = X, residual_out is ignored)
+ *   y = h * gain / sqrt(mean_k h_k^2 + eps)
+ *   codes and scales of the rows of y, as fmm_quantize_rows of unrounded y
+ * dtype (X, residual, residual_out): FMM_DTYPE_BF16 or FMM_DTYPE_F16;
+ * gain_dtype: the same, or FMM_DTYPE_F32.  residual_out may be residual or X
+ * itself (same address and leading dimension).  A row with a value that is
+ * not finite, or whose square is not, has codes 0 and a NaN scale. */
+int fmm_rms_norm_int8(int dtype, int gain_dtype, const void* X, int64_t ldx, const void* residual, int64_t ldr,
+                      const void* gain, int64_t rows, int64_t cols, float eps, void* residual_out, int64_t ldo,
+                      int8_t* codes, int64_t ldq, float* scales, fmm_stream_t stream);
+
+/* C[M,N] (FMM_DTYPE_BF16 or FMM_DTYPE_F16, ldc) =
+ *   (sum_k codes[m,k] * weight_codes[n,k]) * (scales[m] * weight_scales[n]) + bias[n]
+ * the sum exact in 32-bit integers (K <= 131071, else FMM_ERR_TOO_LARGE),
+ * scaled in FP32, bias (dtype, may be NULL) added last, one rounding.
+ * tcgen05 kind::i8 + TMA, persistent. */
+int fmm_linear_int8(int dtype, const int8_t* codes, int64_t ldq, const float* scales,
+                    const int8_t* weight_codes, int64_t ldw, const float* weight_scales, const void* bias,
+                    void* C, int64_t ldc, int64_t M, int64_t K, int64_t N, fmm_stream_t stream);
 
 /* Most SMs any later launch of this library may fill (0 = all, the default;
  * odd values round down to even).  Leaving SMs free lets work on other

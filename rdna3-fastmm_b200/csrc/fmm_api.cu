@@ -21,6 +21,8 @@
 #include "leaf_gemm.cuh"
 #include "reconstruct_tc.cuh"
 #include "reconstruct_staged.cuh"
+#include "int8_rows.cuh"
+#include "int8_gemm.cuh"
 
 // Scratch of fmm_linear_noalloc: the L, Rt and P planes of one call live in
 // this array instead of caller-provided buffers.  It is part of the module, so
@@ -999,6 +1001,134 @@ int launch_leaf_gemm(int rank, const void* L, const void* Rt, int64_t bm, int64_
                                  stream);
 }
 
+// ------------------------------------------------------------------ 8-bit integer linear
+template <class T, class G, bool kNorm, int V, bool kVec>
+int launch_int8_rows(const Int8RowsParams& p, int threads, const DeviceInfo* info, cudaStream_t stream) {
+  const int rows_per_block = p.warps_per_row > 1 ? 1 : threads / 32;
+  const int64_t blocks = ceil_div(p.rows, rows_per_block);
+  // as many blocks as an SM holds at once (2048 threads), then each takes the next rows
+  const int64_t cap = int64_t(usable_sms(info)) * (2048 / threads);
+  const int grid = static_cast<int>(blocks < cap ? blocks : cap);
+  int8_rows_kernel<T, G, kNorm, V, kVec><<<grid, threads, 0, stream>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, kNorm ? "RMS norm (8-bit) launch" : "row quantisation launch");
+  return FMM_OK;
+}
+
+// A row of up to 1024 elements is one warp's (four vectors of 8 a lane), four
+// rows a block; longer rows are a block's, with the fewest vectors a thread
+// that 512 threads cover; beyond 32768 elements (16384 where rows are not
+// aligned: eight vectors spill there) the row is read twice.
+template <class T, class G, bool kNorm, bool kVec>
+int dispatch_int8_rows(Int8RowsParams p, const DeviceInfo* info, cudaStream_t stream) {
+  const int64_t vectors = ceil_div(p.cols, 8);
+  if (vectors <= 128) {
+    p.warps_per_row = 1;
+    if (vectors <= 32) return launch_int8_rows<T, G, kNorm, 1, kVec>(p, 128, info, stream);
+    if (vectors <= 64) return launch_int8_rows<T, G, kNorm, 2, kVec>(p, 128, info, stream);
+    return launch_int8_rows<T, G, kNorm, 4, kVec>(p, 128, info, stream);
+  }
+  auto warps = [&](int v) { return static_cast<int>(ceil_div(ceil_div(vectors, v), 32)); };
+  const int most = kRowsMaxThreads / 32;
+  if (warps(1) <= most) {
+    p.warps_per_row = warps(1);
+    return launch_int8_rows<T, G, kNorm, 1, kVec>(p, 32 * p.warps_per_row, info, stream);
+  }
+  if (warps(2) <= most) {
+    p.warps_per_row = warps(2);
+    return launch_int8_rows<T, G, kNorm, 2, kVec>(p, 32 * p.warps_per_row, info, stream);
+  }
+  if (warps(4) <= most) {
+    p.warps_per_row = warps(4);
+    return launch_int8_rows<T, G, kNorm, 4, kVec>(p, 32 * p.warps_per_row, info, stream);
+  }
+  if constexpr (kVec) {
+    if (warps(8) <= most) {
+      p.warps_per_row = warps(8);
+      return launch_int8_rows<T, G, kNorm, 8, kVec>(p, 32 * p.warps_per_row, info, stream);
+    }
+  }
+  p.warps_per_row = most;
+  return launch_int8_rows<T, G, kNorm, 0, kVec>(p, kRowsMaxThreads, info, stream);
+}
+
+// kVec: every row of every tensor starts on a vector's boundary.
+template <class T, class G, bool kNorm>
+int run_int8_rows(const Int8RowsParams& p, cudaStream_t stream) {
+  if (p.rows == 0) return FMM_OK;
+  DeviceInfo* info = nullptr;
+  if (int rc = device_info(&info)) return rc;
+  constexpr int64_t kPer16 = 16 / sizeof(T);
+  bool vec = aligned(p.x, 16) && p.ldx % kPer16 == 0 && aligned(p.codes, 8) && p.ldq % 8 == 0;
+  if (kNorm) vec = vec && aligned(p.gain, 16);
+  if (p.residual != nullptr)
+    vec = vec && aligned(p.residual, 16) && p.ldr % kPer16 == 0 && aligned(p.residual_out, 16) && p.ldo % kPer16 == 0;
+  return vec ? dispatch_int8_rows<T, G, kNorm, true>(p, info, stream)
+             : dispatch_int8_rows<T, G, kNorm, false>(p, info, stream);
+}
+
+int check_rows(int64_t rows, int64_t cols) {
+  if (rows < 0 || cols < 1) return fail(FMM_ERR_INVALID_ARGUMENT, "rows must not be negative and columns positive");
+  if (cols > (int64_t(1) << 30)) return fail(FMM_ERR_TOO_LARGE, "rows of more than 2^30 elements");
+  return FMM_OK;
+}
+
+// 8-bit codes [rows][ld] as a 2-D map over (k, row); box = 128 codes (one
+// swizzled 128-byte row) x box_rows.
+int codes_map(CUtensorMap* map, const void* base, int64_t k, int64_t rows, int64_t ld, uint32_t box_rows) {
+  PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+  if (int rc = tensor_map_encoder(&encode)) return rc;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(kI8BlockK), box_rows};
+  cuuint32_t elem[2] = {1, 1};
+  CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, elem,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FMM_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string(r) + ")");
+  return FMM_OK;
+}
+
+constexpr size_t kI8MaxSmem = 232448;
+
+template <bool kBf16>
+int launch_linear_int8(const int8_t* codes, int64_t ldq, const int8_t* weight_codes, int64_t ldw,
+                       Int8LinearParams p, cudaStream_t stream) {
+  static bool configured[kMaxDevices] = {};
+  DeviceInfo* info = nullptr;
+  if (int rc = device_info(&info)) return rc;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  p.tok = static_cast<int32_t>(p.M >= 256 ? 256 : round_up(p.M, 16));
+  p.tmem_cols = 32;
+  while (p.tmem_cols < static_cast<uint32_t>(p.tok)) p.tmem_cols *= 2;
+  const int64_t tiles_m = ceil_div(p.M, p.tok), tiles_n = ceil_div(p.N, kI8TileN);
+  if (tiles_m * tiles_n > (int64_t(1) << 30)) return fail(FMM_ERR_TOO_LARGE, "too many tiles");
+  p.tiles_m = static_cast<int32_t>(tiles_m);
+  p.tiles_n = static_cast<int32_t>(tiles_n);
+  const size_t stage = kI8WBytes + size_t(p.tok) * kI8BlockK;
+  const size_t control = 1024 + 8 * (2 * kI8MaxStages + 4);
+  p.stages = kI8MaxStages;
+  while (p.stages * stage + control > kI8MaxSmem) --p.stages;
+  const size_t smem = p.stages * stage + control;
+  p.timeout_ns = g_timeout_ns;
+  CUtensorMap map_w, map_q;
+  if (int rc = codes_map(&map_w, weight_codes, p.K, p.N, ldw, kI8TileN)) return rc;
+  if (int rc = codes_map(&map_q, codes, p.K, p.M, ldq, static_cast<uint32_t>(p.tok))) return rc;
+  {
+    std::lock_guard<std::mutex> lock(g_device_mutex);
+    if (int rc = ensure_smem_attribute(configured[dev], int8_linear_kernel<kBf16>, kI8MaxSmem)) return rc;
+  }
+  const int64_t tiles = tiles_m * tiles_n;
+  const int sms = usable_sms(info);
+  const int grid = static_cast<int>(tiles < sms ? tiles : sms);
+  int8_linear_kernel<kBf16><<<grid, kI8Threads, smem, stream>>>(map_w, map_q, p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "8-bit linear launch");
+  return FMM_OK;
+}
+
 // Device address of g_noalloc_scratch on the current device.  In host code the
 // array's name is only a host-side stand-in, so the address is looked up once
 // per device (with that device current) and cached.
@@ -1195,6 +1325,102 @@ int fmm_linear_noalloc(int scheme, const void* A, const void* W, const void* bia
   // in the same call (pitch padding included), so nothing is cleared first.
   return fmm_linear(scheme, FMM_DTYPE_BF16, A, W, bias, C, M, K, N, bytes, bytes + left,
                     bytes + left + right, 0u, stream);
+}
+
+// ------------------------------------------------------------------ 8-bit integer linear
+int fmm_quantize_rows(int dtype, const void* X, int64_t rows, int64_t cols, int64_t ldx, int8_t* codes,
+                      int64_t ldq, float* scales, fmm_stream_t stream) {
+  if (dtype != FMM_DTYPE_BF16 && dtype != FMM_DTYPE_F16 && dtype != FMM_DTYPE_F32)
+    return fail(FMM_ERR_UNSUPPORTED, "dtype must be FMM_DTYPE_BF16, FMM_DTYPE_F16 or FMM_DTYPE_F32");
+  if (int rc = check_rows(rows, cols)) return rc;
+  if (rows > 0 && (X == nullptr || codes == nullptr || scales == nullptr))
+    return fail(FMM_ERR_INVALID_ARGUMENT, "null pointer");
+  if (ldx < cols || ldq < cols) return fail(FMM_ERR_INVALID_ARGUMENT, "ldx or ldq < cols");
+  if (!aligned(X, dtype == FMM_DTYPE_F32 ? 4 : 2) || !aligned(scales, 4))
+    return fail(FMM_ERR_MISALIGNED, "X and scales must be aligned to their elements");
+  Int8RowsParams p = {};
+  p.x = X;
+  p.codes = codes;
+  p.scales = scales;
+  p.rows = rows;
+  p.ldx = ldx;
+  p.ldq = ldq;
+  p.cols = static_cast<int32_t>(cols);
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == FMM_DTYPE_F32) return run_int8_rows<float, float, false>(p, s);
+  if (dtype == FMM_DTYPE_F16) return run_int8_rows<__half, __half, false>(p, s);
+  return run_int8_rows<__nv_bfloat16, __nv_bfloat16, false>(p, s);
+}
+
+int fmm_rms_norm_int8(int dtype, int gain_dtype, const void* X, int64_t ldx, const void* residual, int64_t ldr,
+                      const void* gain, int64_t rows, int64_t cols, float eps, void* residual_out, int64_t ldo,
+                      int8_t* codes, int64_t ldq, float* scales, fmm_stream_t stream) {
+  if (dtype != FMM_DTYPE_BF16 && dtype != FMM_DTYPE_F16)
+    return fail(FMM_ERR_UNSUPPORTED, "dtype must be FMM_DTYPE_BF16 or FMM_DTYPE_F16");
+  if (gain_dtype != dtype && gain_dtype != FMM_DTYPE_F32)
+    return fail(FMM_ERR_UNSUPPORTED, "the gain has the dtype of X or FMM_DTYPE_F32");
+  if (int rc = check_rows(rows, cols)) return rc;
+  if (!(eps >= 0.0f) || std::isinf(eps)) return fail(FMM_ERR_INVALID_ARGUMENT, "eps must be finite and not negative");
+  if (rows > 0 && (X == nullptr || gain == nullptr || codes == nullptr || scales == nullptr))
+    return fail(FMM_ERR_INVALID_ARGUMENT, "null pointer");
+  if (residual != nullptr && residual_out == nullptr)
+    return fail(FMM_ERR_INVALID_ARGUMENT, "a residual needs residual_out");
+  if (ldx < cols || ldq < cols || (residual != nullptr && (ldr < cols || ldo < cols)))
+    return fail(FMM_ERR_INVALID_ARGUMENT, "a leading dimension is less than cols");
+  if (!aligned(X, 2) || !aligned(residual, 2) || !aligned(residual_out, 2) || !aligned(scales, 4) ||
+      !aligned(gain, gain_dtype == FMM_DTYPE_F32 ? 4 : 2))
+    return fail(FMM_ERR_MISALIGNED, "operands must be aligned to their elements");
+  Int8RowsParams p = {};
+  p.x = X;
+  p.residual = residual;
+  p.residual_out = residual != nullptr ? residual_out : nullptr;
+  p.gain = gain;
+  p.codes = codes;
+  p.scales = scales;
+  p.rows = rows;
+  p.ldx = ldx;
+  p.ldr = ldr;
+  p.ldo = ldo;
+  p.ldq = ldq;
+  p.cols = static_cast<int32_t>(cols);
+  p.eps = eps;
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (gain_dtype == FMM_DTYPE_F32)
+    return dtype == FMM_DTYPE_F16 ? run_int8_rows<__half, float, true>(p, s)
+                                  : run_int8_rows<__nv_bfloat16, float, true>(p, s);
+  return dtype == FMM_DTYPE_F16 ? run_int8_rows<__half, __half, true>(p, s)
+                                : run_int8_rows<__nv_bfloat16, __nv_bfloat16, true>(p, s);
+}
+
+int fmm_linear_int8(int dtype, const int8_t* codes, int64_t ldq, const float* scales,
+                    const int8_t* weight_codes, int64_t ldw, const float* weight_scales, const void* bias,
+                    void* C, int64_t ldc, int64_t M, int64_t K, int64_t N, fmm_stream_t stream) {
+  if (dtype != FMM_DTYPE_BF16 && dtype != FMM_DTYPE_F16)
+    return fail(FMM_ERR_UNSUPPORTED, "dtype must be FMM_DTYPE_BF16 or FMM_DTYPE_F16");
+  if (M < 0 || K < 1 || N < 1)
+    return fail(FMM_ERR_INVALID_ARGUMENT, "M must not be negative, K and N positive");
+  if (K > 131071) return fail(FMM_ERR_TOO_LARGE, "K beyond 131071 could leave the 32-bit sum");
+  if (M > (int64_t(1) << 30) || N > (int64_t(1) << 30)) return fail(FMM_ERR_TOO_LARGE, "M or N beyond 2^30");
+  if (ldq < K || ldw < K || ldc < N) return fail(FMM_ERR_INVALID_ARGUMENT, "a leading dimension is too small");
+  if (M == 0) return FMM_OK;
+  if (codes == nullptr || scales == nullptr || weight_codes == nullptr || weight_scales == nullptr || C == nullptr)
+    return fail(FMM_ERR_INVALID_ARGUMENT, "null pointer");
+  if (!aligned(codes, 16) || !aligned(weight_codes, 16) || ldq % 16 != 0 || ldw % 16 != 0)
+    return fail(FMM_ERR_MISALIGNED, "code rows must start on 16-byte boundaries");
+  if (!aligned(scales, 4) || !aligned(weight_scales, 4) || !aligned(bias, 2) || !aligned(C, 2))
+    return fail(FMM_ERR_MISALIGNED, "operands must be aligned to their elements");
+  Int8LinearParams p = {};
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.ldc = ldc;
+  p.token_scales = scales;
+  p.channel_scales = weight_scales;
+  p.bias = bias;
+  p.out = C;
+  const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return dtype == FMM_DTYPE_BF16 ? launch_linear_int8<true>(codes, ldq, weight_codes, ldw, p, s)
+                                 : launch_linear_int8<false>(codes, ldq, weight_codes, ldw, p, s);
 }
 
 // ------------------------------------------------------------------ peer memory (IPC)

@@ -1,0 +1,515 @@
+"""8-bit integer linear: row quantisation, RMS norm with an 8-bit output, and
+the product of the codes.
+
+A quantised matrix is a pair of 8-bit codes and FP32 scales, one for each row:
+a token of the activations, an output channel of the weight.  The value of a
+code is ``code * scale``; codes are symmetric, ``round(127 x / max|x|)``.
+
+* ``quantize_rows(x)`` -- codes and scales of BF16, FP16 or FP32 rows;
+* ``rms_norm_int8(x, weight, residual, eps)`` -- adds the residual, normalises
+  and quantises in one pass, and returns the new residual;
+* ``linear_int8(codes, scales, weight_codes, weight_scales, bias)`` -- the
+  linear, exact 32-bit sums scaled once;
+* ``Int8Plan`` -- a plan in the manner of ``runtime.Rank7Plan``: packs a
+  weight once, keeps a workspace, runs ``x -> codes -> product`` and
+  ``x, residual -> norm -> codes -> product``;
+* ``torch.ops.rdna3_fastmm.{quantize_rows_int8, rms_norm_int8, linear_int8}``.
+
+Code rows start on 16-byte boundaries: a ``[rows, K]`` tensor of codes made
+here is a view of ``[rows, round_up(K, 16)]`` storage.  Calls are queued on the
+current stream of the operands' device; with buffers given for their outputs
+they allocate nothing and capture into CUDA graphs.  They do not support
+autograd: an operand that requires a gradient is refused while gradients are
+enabled.  The reference has no quantised operator.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _native
+from .runtime import _LinearPlan, _round_up
+
+__all__ = [
+    "Int8Rows",
+    "NormedInt8Rows",
+    "Int8PackedWeight",
+    "Int8Workspace",
+    "Int8Plan",
+    "quantize_rows",
+    "rms_norm_int8",
+    "linear_int8",
+    "empty_codes",
+]
+
+CODE_ALIGNMENT = 16
+MAX_INNER = 131071  # 2^14 a product of two codes of -128, sums below 2^31
+_HALF_TYPES = (torch.bfloat16, torch.float16)
+
+
+class Int8Rows(NamedTuple):
+    codes: torch.Tensor  # int8, [..., K]
+    scales: torch.Tensor  # float32, [...]
+
+
+class NormedInt8Rows(NamedTuple):
+    codes: torch.Tensor
+    scales: torch.Tensor
+    residual: torch.Tensor | None  # x + residual in x's type; None without a residual
+
+
+def empty_codes(shape: tuple[int, ...], device: torch.device) -> torch.Tensor:
+    """Uninitialised codes of ``shape`` whose rows start on 16-byte boundaries."""
+    inner = shape[-1]
+    pitch = _round_up(inner, CODE_ALIGNMENT)
+    storage = torch.empty((*shape[:-1], pitch), device=device, dtype=torch.int8)
+    return storage if pitch == inner else storage[..., :inner]
+
+
+# ---------------------------------------------------------------- operands
+class _Rows(NamedTuple):
+    """A tensor as rows: address, count, length and step in elements."""
+
+    ptr: int
+    rows: int
+    inner: int
+    pitch: int
+    itemsize: int
+    keep: torch.Tensor  # holds the memory where the rows had to be copied
+
+
+def _flat(tensor: torch.Tensor) -> tuple[int, int, int] | None:
+    """(rows, inner, pitch) where the leading dimensions are rows a constant
+    step apart and the last dimension is dense, else None."""
+    shape = tensor.shape
+    inner = shape[-1]
+    if tensor.ndim == 1:
+        rows, pitch = 1, inner
+    elif tensor.ndim == 2:
+        rows, pitch = shape[0], tensor.stride(0)
+    else:
+        rows, pitch, step = 1, None, None
+        for size, stride in zip(reversed(shape[:-1]), reversed(tensor.stride()[:-1])):
+            if size == 1:
+                continue
+            if pitch is None:
+                pitch = stride
+            elif stride != step:
+                return None
+            rows *= size
+            step = stride * size
+        if pitch is None:
+            pitch = inner
+    if inner > 1 and tensor.stride(-1) != 1:
+        return None
+    if rows <= 1:
+        pitch = _round_up(inner, CODE_ALIGNMENT)  # no second row to reach
+    elif pitch < inner:
+        return None
+    return rows, inner, pitch
+
+
+def _input_rows(tensor: torch.Tensor) -> _Rows:
+    flat = _flat(tensor)
+    if flat is None:
+        tensor = tensor.contiguous()
+        flat = _flat(tensor)
+    return _Rows(tensor.data_ptr(), *flat, tensor.element_size(), tensor)
+
+
+def _output_rows(tensor: torch.Tensor, shape: torch.Size, dtype: torch.dtype, device: torch.device,
+                 name: str) -> _Rows:
+    if tensor.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(tensor.shape)}, expected {tuple(shape)}")
+    if tensor.device != device or tensor.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype} on {device}")
+    _refuse_grad(tensor)
+    flat = _flat(tensor)
+    if flat is None:
+        raise ValueError(f"{name} must have dense rows a constant step apart")
+    return _Rows(tensor.data_ptr(), *flat, tensor.element_size(), tensor)
+
+
+def _input_scales(tensor: torch.Tensor, shape: torch.Size, device: torch.device, name: str) -> torch.Tensor:
+    if tensor.shape != shape:
+        raise ValueError(f"{name} has shape {tuple(tensor.shape)}, expected {tuple(shape)}")
+    if tensor.device != device or tensor.dtype != torch.float32:
+        raise ValueError(f"{name} must be float32 on {device}")
+    _refuse_grad(tensor)
+    return tensor.contiguous()
+
+
+def _output_scales(tensor: torch.Tensor, shape: torch.Size, device: torch.device) -> torch.Tensor:
+    if tensor.shape != shape:
+        raise ValueError(f"scales has shape {tuple(tensor.shape)}, expected {tuple(shape)}")
+    if tensor.device != device or tensor.dtype != torch.float32 or not tensor.is_contiguous():
+        raise ValueError(f"scales must be contiguous float32 on {device}")
+    _refuse_grad(tensor)
+    return tensor
+
+
+def _refuse_grad(tensor: torch.Tensor) -> None:
+    if tensor.requires_grad and torch.is_grad_enabled():
+        raise ValueError("the B200 8-bit operators do not support autograd")
+
+
+def _require_cuda(tensor: torch.Tensor, name: str) -> None:
+    if tensor.device.type != "cuda":
+        raise ValueError(f"{name} must be a CUDA tensor")
+
+
+def _rows_overlap(a: _Rows, b: _Rows) -> bool:
+    """Whether two row operands share a byte."""
+    if a.rows == 0 or b.rows == 0:
+        return False
+    width_a, width_b = a.inner * a.itemsize, b.inner * b.itemsize
+    step_a, step_b = a.pitch * a.itemsize, b.pitch * b.itemsize
+    if a.ptr >= b.ptr + (b.rows - 1) * step_b + width_b or b.ptr >= a.ptr + (a.rows - 1) * step_a + width_a:
+        return False
+    if a.rows > 1 and b.rows > 1 and step_a == step_b:
+        # columns of one buffer: apart if their byte ranges within a step are
+        offset = (b.ptr - a.ptr) % step_a
+        return offset < width_a or offset + width_b > step_a
+    return True
+
+
+def _row_vector(tensor: torch.Tensor) -> _Rows:
+    n = tensor.numel()
+    return _Rows(tensor.data_ptr(), 1 if n else 0, n, n, tensor.element_size(), tensor)
+
+
+def _same_rows(a: _Rows, b: _Rows) -> bool:
+    return a.ptr == b.ptr and a.pitch == b.pitch
+
+
+def _refuse_overlap(outputs: tuple[_Rows, ...], inputs: tuple[_Rows, ...]) -> None:
+    for i, out in enumerate(outputs):
+        for other in outputs[i + 1:] + inputs:
+            if _rows_overlap(out, other):
+                raise ValueError("output storage must not overlap inputs or other outputs")
+
+
+def _launch(device: torch.device, function, *args) -> None:
+    """Call ``function`` with ``device`` current, on its current stream."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        function(*args, torch._C._cuda_getCurrentRawStream(index))
+        return
+    with torch.cuda.device(index):
+        function(*args, torch._C._cuda_getCurrentRawStream(index))
+
+
+# ---------------------------------------------------------------- operators
+def quantize_rows(x: torch.Tensor, *, codes: torch.Tensor | None = None,
+                  scales: torch.Tensor | None = None) -> Int8Rows:
+    """8-bit codes and scales of the rows ``x[..., K]`` (BF16, FP16 or FP32).
+
+    ``codes[..., k] = round_half_even(127 x[..., k] / a)`` and ``scales = a / 127``
+    with ``a`` the row's largest magnitude.  A row of zeros has scale 0; a row
+    with an infinity or a NaN has codes 0 and scale NaN.  ``codes`` and
+    ``scales`` are written and returned where given."""
+    _require_cuda(x, "x")
+    dtype = _native.row_dtype_id(x.dtype)
+    if x.ndim < 1 or x.shape[-1] < 1:
+        raise ValueError("x must have a last dimension of at least one element")
+    _refuse_grad(x)
+    source = _input_rows(x)
+    codes = empty_codes(x.shape, x.device) if codes is None else codes
+    scales = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32) if scales is None else scales
+    q = _output_rows(codes, x.shape, torch.int8, x.device, "codes")
+    _output_scales(scales, x.shape[:-1], x.device)
+    _refuse_overlap((q, _row_vector(scales)), (source,))
+    if source.rows:
+        _launch(x.device, _native.quantize_rows, dtype, source.ptr, source.rows, source.inner, source.pitch, q.ptr,
+                q.pitch, scales.data_ptr())
+    return Int8Rows(codes, scales)
+
+
+def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-6, *,
+                  codes: torch.Tensor | None = None, scales: torch.Tensor | None = None,
+                  residual_out: torch.Tensor | None = None) -> NormedInt8Rows:
+    """RMS norm of ``h = x + residual`` with an 8-bit output.
+
+    ``h`` is rounded to ``x``'s type (BF16 or FP16), returned as the new
+    residual, and read by the norm; ``y = h * weight / sqrt(mean(h^2) + eps)``
+    is quantised unrounded as by ``quantize_rows``.  ``weight[K]`` has ``x``'s
+    type or FP32.  ``residual_out`` may be ``residual`` or ``x`` itself, which
+    updates the stream in place."""
+    _require_cuda(x, "x")
+    if x.dtype not in _HALF_TYPES:
+        raise ValueError(f"rms_norm_int8 takes BF16 or FP16 rows, not {x.dtype}")
+    if x.ndim < 1 or x.shape[-1] < 1:
+        raise ValueError("x must have a last dimension of at least one element")
+    if weight.shape != x.shape[-1:]:
+        raise ValueError(f"weight has shape {tuple(weight.shape)}, expected {tuple(x.shape[-1:])}")
+    if weight.device != x.device or weight.dtype not in (x.dtype, torch.float32):
+        raise ValueError("weight must have x's dtype or float32, on x's device")
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError("eps must be finite and not negative")
+    if residual is None and residual_out is not None:
+        raise ValueError("residual_out needs a residual")
+    _refuse_grad(x)
+    _refuse_grad(weight)
+    source = _input_rows(x)
+    gain = _row_vector(weight.contiguous())
+    inputs = [source, gain]
+    codes = empty_codes(x.shape, x.device) if codes is None else codes
+    scales = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32) if scales is None else scales
+    q = _output_rows(codes, x.shape, torch.int8, x.device, "codes")
+    _output_scales(scales, x.shape[:-1], x.device)
+    outputs = [q, _row_vector(scales)]
+    added, stream_out = None, None
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
+            raise ValueError("residual must have x's shape, dtype and device")
+        _refuse_grad(residual)
+        added = _input_rows(residual)
+        if residual_out is None:
+            residual_out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+        stream_out = _output_rows(residual_out, x.shape, x.dtype, x.device, "residual_out")
+        for other in (source, added):
+            if not _same_rows(stream_out, other) and _rows_overlap(stream_out, other):
+                raise ValueError("residual_out must be residual, x or storage of its own")
+        _refuse_overlap((stream_out,), (gain, *outputs))
+        inputs.append(added)
+    _refuse_overlap(tuple(outputs), tuple(inputs))
+    if source.rows:
+        _launch(x.device, _native.rms_norm_int8, _native.row_dtype_id(x.dtype), _native.row_dtype_id(weight.dtype),
+                source.ptr, source.pitch, None if added is None else added.ptr, 0 if added is None else added.pitch,
+                gain.ptr, source.rows, source.inner, eps, None if stream_out is None else stream_out.ptr,
+                0 if stream_out is None else stream_out.pitch, q.ptr, q.pitch, scales.data_ptr())
+    return NormedInt8Rows(codes, scales, residual_out)
+
+
+def linear_int8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.Tensor, weight_scales: torch.Tensor,
+                bias: torch.Tensor | None = None, *, dtype: torch.dtype | None = None,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """``(codes * scales) @ (weight_codes * weight_scales).T + bias``.
+
+    ``codes[..., K]`` with ``scales[...]``, ``weight_codes[N, K]`` with
+    ``weight_scales[N]``; the output ``[..., N]`` is BF16 or FP16 (``dtype``,
+    or ``out``'s or ``bias``'s; BF16 where none says).  Products are summed
+    exactly in 32-bit integers (``K`` up to 131071), scaled and biased in FP32
+    and rounded once.  Code rows must start on 16-byte boundaries, as
+    ``quantize_rows``, ``rms_norm_int8`` and ``empty_codes`` make them."""
+    _require_cuda(codes, "codes")
+    device = codes.device
+    if codes.dtype != torch.int8 or weight_codes.dtype != torch.int8 or weight_codes.device != device:
+        raise ValueError("codes and weight_codes must be int8 tensors of one device")
+    if codes.ndim < 1 or weight_codes.ndim != 2 or codes.shape[-1] != weight_codes.shape[1]:
+        raise ValueError("codes and weight_codes shapes do not form a linear")
+    columns, inner = weight_codes.shape
+    if columns < 1 or inner < 1:
+        raise ValueError("matrix dimensions must be positive")
+    if inner > MAX_INNER:
+        raise ValueError(f"K = {inner} could leave the 32-bit sum (at most {MAX_INNER})")
+    if dtype is None:
+        dtype = out.dtype if out is not None else bias.dtype if bias is not None else torch.bfloat16
+    if dtype not in _HALF_TYPES:
+        raise ValueError(f"linear_int8 writes BF16 or FP16, not {dtype}")
+    q, w = _flat(codes), _flat(weight_codes)
+    if q is None or w is None:
+        raise ValueError("codes must have dense rows a constant step apart")
+    token_scales = _input_scales(scales, codes.shape[:-1], device, "scales")
+    channel_scales = _input_scales(weight_scales, weight_codes.shape[:1], device, "weight_scales")
+    if bias is not None:
+        if bias.shape != (columns,) or bias.dtype != dtype or bias.device != device:
+            raise ValueError(f"bias must be {dtype} [N] on the codes' device")
+        _refuse_grad(bias)
+        bias = bias.contiguous()
+    shape = torch.Size((*codes.shape[:-1], columns))
+    fresh = out is None
+    if fresh:
+        out = torch.empty(shape, device=device, dtype=dtype)
+    result = _output_rows(out, shape, dtype, device, "out")
+    rows, _, pitch = q
+    if not fresh:
+        inputs = [_Rows(codes.data_ptr(), *q, 1, codes), _Rows(weight_codes.data_ptr(), *w, 1, weight_codes),
+                  _row_vector(token_scales), _row_vector(channel_scales)]
+        if bias is not None:
+            inputs.append(_row_vector(bias))
+        _refuse_overlap((result,), tuple(inputs))
+    if rows:
+        _launch(device, _native.linear_int8, _native.row_dtype_id(dtype), codes.data_ptr(), pitch,
+                token_scales.data_ptr(), weight_codes.data_ptr(), w[2], channel_scales.data_ptr(),
+                None if bias is None else bias.data_ptr(), result.ptr, result.pitch, rows, inner, columns)
+    return out
+
+
+# ---------------------------------------------------------------- plan
+@dataclass
+class Int8Workspace:
+    algorithm: str
+    output_dtype: torch.dtype
+    codes: torch.Tensor  # [rows, K] of 16-byte aligned rows
+    scales: torch.Tensor  # [rows]
+
+
+@dataclass(frozen=True)
+class Int8PackedWeight:
+    algorithm: str
+    source_dtype: torch.dtype
+    codes: torch.Tensor  # [N, K] of 16-byte aligned rows
+    scales: torch.Tensor  # [N]
+    source_shape: tuple[int, int]
+
+
+class Int8Plan:
+    """8-bit linear of ``rows x inner`` inputs and a ``columns x inner`` weight,
+    used as the reduced-rank plans are: pack the weight once, keep a workspace,
+    run.  A packed weight serves plans of any row count; two streams (or two
+    captured graphs that may run together) need a workspace each."""
+
+    algorithm = "int8-v1"
+    _ensure_memory_budget = _LinearPlan._ensure_memory_budget
+
+    def __init__(self, rows: int, inner: int, columns: int, device: torch.device,
+                 dtype: torch.dtype = torch.bfloat16) -> None:
+        device = torch.device(device)
+        if device.type != "cuda" or torch.version.cuda is None or not torch.cuda.is_available():
+            raise ValueError("the B200 backend requires a CUDA sm_100 device")
+        if dtype not in _HALF_TYPES:
+            raise ValueError(f"{self.algorithm} does not support {dtype} inputs")
+        if min(rows, inner, columns) < 1:
+            raise ValueError("matrix dimensions must be positive")
+        if inner > MAX_INNER:
+            raise ValueError(f"K = {inner} could leave the 32-bit sum (at most {MAX_INNER})")
+        index = torch.cuda.current_device() if device.index is None else device.index
+        self.device = torch.device("cuda", index)
+        self.dtype = dtype
+        self.rows, self.inner, self.columns = rows, inner, columns
+
+    @property
+    def workspace_bytes(self) -> int:
+        return self.rows * (_round_up(self.inner, CODE_ALIGNMENT) + 4)
+
+    @property
+    def packed_weight_bytes(self) -> int:
+        return self.columns * (_round_up(self.inner, CODE_ALIGNMENT) + 4)
+
+    def allocate_workspace(self, max_free_memory_fraction: float = 0.75) -> Int8Workspace:
+        self._ensure_memory_budget(self.workspace_bytes, max_free_memory_fraction, f"{self.algorithm} workspace")
+        return Int8Workspace(self.algorithm, self.dtype, empty_codes((self.rows, self.inner), self.device),
+                             torch.empty((self.rows,), device=self.device, dtype=torch.float32))
+
+    def pack_weight(self, weight: torch.Tensor, max_free_memory_fraction: float = 0.75) -> Int8PackedWeight:
+        """Quantise ``weight[N, K]`` (the plan's type or FP32) once, a scale for
+        each output channel, into an immutable snapshot."""
+        if tuple(weight.shape) != (self.columns, self.inner):
+            raise ValueError(f"weight matrix has shape {tuple(weight.shape)}, "
+                             f"expected {(self.columns, self.inner)}")
+        if weight.device != self.device or weight.dtype not in (self.dtype, torch.float32):
+            raise ValueError("weight matrix device or dtype does not match the plan")
+        self._ensure_memory_budget(self.packed_weight_bytes, max_free_memory_fraction,
+                                   f"{self.algorithm} packed Linear weight")
+        codes, scales = quantize_rows(weight)
+        return Int8PackedWeight(self.algorithm, self.dtype, codes, scales, (self.columns, self.inner))
+
+    def run_linear_packed(self, input_tensor: torch.Tensor, weight: Int8PackedWeight, workspace: Int8Workspace,
+                          bias: torch.Tensor | None = None, output: torch.Tensor | None = None) -> torch.Tensor:
+        """``F.linear(input, weight, bias)``: tokens to codes, codes to output."""
+        self._validate_input(input_tensor)
+        self._validate_packed(weight)
+        self._validate_workspace(workspace)
+        self._refuse_output(output, input_tensor)
+        self._refuse_weight(workspace, weight)
+        quantize_rows(input_tensor, codes=workspace.codes, scales=workspace.scales)
+        return linear_int8(workspace.codes, workspace.scales, weight.codes, weight.scales, bias, dtype=self.dtype,
+                           out=output)
+
+    def run_norm_linear_packed(self, input_tensor: torch.Tensor, norm_weight: torch.Tensor, weight: Int8PackedWeight,
+                               workspace: Int8Workspace, residual: torch.Tensor | None = None, eps: float = 1e-6,
+                               bias: torch.Tensor | None = None, output: torch.Tensor | None = None,
+                               residual_output: torch.Tensor | None = None,
+                               ) -> tuple[torch.Tensor, torch.Tensor | None]:
+        """``F.linear(rms_norm(input + residual), weight, bias)`` and the new
+        residual (``None`` without one)."""
+        self._validate_input(input_tensor)
+        self._validate_packed(weight)
+        self._validate_workspace(workspace)
+        self._refuse_output(output, input_tensor, norm_weight, residual, residual_output)
+        self._refuse_output(residual_output, weight.codes, weight.scales, bias)
+        self._refuse_weight(workspace, weight)
+        stream = rms_norm_int8(input_tensor, norm_weight, residual, eps, codes=workspace.codes,
+                               scales=workspace.scales, residual_out=residual_output).residual
+        result = linear_int8(workspace.codes, workspace.scales, weight.codes, weight.scales, bias, dtype=self.dtype,
+                             out=output)
+        return result, stream
+
+    # ------------------------------------------------------------------ checks
+    def _validate_input(self, tensor: torch.Tensor) -> None:
+        if tuple(tensor.shape) != (self.rows, self.inner):
+            raise ValueError(f"left matrix has shape {tuple(tensor.shape)}, expected {(self.rows, self.inner)}")
+        if tensor.device != self.device or tensor.dtype != self.dtype:
+            raise ValueError("left matrix device or dtype does not match the plan")
+
+    def _validate_packed(self, packed: Int8PackedWeight) -> None:
+        if (not isinstance(packed, Int8PackedWeight) or packed.algorithm != self.algorithm
+                or packed.source_dtype != self.dtype or packed.codes.device != self.device):
+            raise ValueError("packed Linear weight does not match the plan")
+        if packed.source_shape != (self.columns, self.inner) or tuple(packed.codes.shape) != packed.source_shape:
+            raise ValueError("packed Linear weight shape does not match the plan")
+
+    def _validate_workspace(self, workspace: Int8Workspace) -> None:
+        if (not isinstance(workspace, Int8Workspace) or workspace.algorithm != self.algorithm
+                or workspace.output_dtype != self.dtype or workspace.codes.device != self.device
+                or tuple(workspace.codes.shape) != (self.rows, self.inner)):
+            raise ValueError("workspace does not match the plan")
+
+    @staticmethod
+    def _refuse_weight(workspace: Int8Workspace, weight: Int8PackedWeight) -> None:
+        for buffer in (workspace.codes, workspace.scales):
+            for packed in (weight.codes, weight.scales):
+                if _rows_overlap(_input_rows(buffer), _input_rows(packed)):
+                    raise ValueError("work buffers must not overlap")
+
+    @staticmethod
+    def _refuse_output(output: torch.Tensor | None, *tensors: torch.Tensor | None) -> None:
+        """What the first kernel reads or writes must outlive the second's output."""
+        if output is None or _flat(output) is None:
+            return  # a malformed output is refused where it is used
+        rows = _input_rows(output)
+        for tensor in tensors:
+            if tensor is not None and _rows_overlap(rows, _input_rows(tensor)):
+                raise ValueError("output storage must not overlap inputs or workspace")
+
+
+# ---------------------------------------------------------------- torch.library
+@torch.library.custom_op("rdna3_fastmm::quantize_rows_int8", mutates_args=(), device_types="cuda")
+def quantize_rows_int8_op(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    codes, scales = quantize_rows(x)
+    return codes, scales
+
+
+@torch.library.custom_op("rdna3_fastmm::rms_norm_int8", mutates_args=(), device_types="cuda")
+def rms_norm_int8_op(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None,
+                     eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    codes, scales, stream = rms_norm_int8(x, weight, residual, eps)
+    # without a residual there is no new one: an operator cannot return None
+    return codes, scales, x.new_empty((0,)) if stream is None else stream
+
+
+@torch.library.custom_op("rdna3_fastmm::linear_int8", mutates_args=(), device_types="cuda")
+def linear_int8_op(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.Tensor,
+                   weight_scales: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                   dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    return linear_int8(codes, scales, weight_codes, weight_scales, bias, dtype=dtype)
+
+
+@quantize_rows_int8_op.register_fake
+def _(x):
+    return empty_codes(x.shape, x.device), x.new_empty(x.shape[:-1], dtype=torch.float32)
+
+
+@rms_norm_int8_op.register_fake
+def _(x, weight, residual=None, eps=1e-6):
+    stream = x.new_empty((0,)) if residual is None else x.new_empty(x.shape)
+    return empty_codes(x.shape, x.device), x.new_empty(x.shape[:-1], dtype=torch.float32), stream
+
+
+@linear_int8_op.register_fake
+def _(codes, scales, weight_codes, weight_scales, bias=None, dtype=torch.bfloat16):
+    return codes.new_empty((*codes.shape[:-1], weight_codes.shape[0]), dtype=dtype)
