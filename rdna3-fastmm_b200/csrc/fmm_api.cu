@@ -1006,8 +1006,8 @@ template <class T, class G, bool kNorm, int V, bool kVec>
 int launch_int8_rows(const Int8RowsParams& p, int threads, const DeviceInfo* info, cudaStream_t stream) {
   const int rows_per_block = p.warps_per_row > 1 ? 1 : threads / 32;
   const int64_t blocks = ceil_div(p.rows, rows_per_block);
-  // as many blocks as an SM holds at once (2048 threads), then each takes the next rows
-  const int64_t cap = int64_t(usable_sms(info)) * (2048 / threads);
+  // the blocks that an SM is sure to hold at once (64 registers a thread); each takes row after row
+  const int64_t cap = int64_t(usable_sms(info)) * (kRowsMaxThreads / threads);
   const int grid = static_cast<int>(blocks < cap ? blocks : cap);
   int8_rows_kernel<T, G, kNorm, V, kVec><<<grid, threads, 0, stream>>>(p);
   cudaError_t e = cudaGetLastError();
@@ -1015,13 +1015,84 @@ int launch_int8_rows(const Int8RowsParams& p, int threads, const DeviceInfo* inf
   return FMM_OK;
 }
 
-// A row of up to 1024 elements is one warp's (four vectors of 8 a lane), four
-// rows a block; longer rows are a block's, with the fewest vectors a thread
-// that 512 threads cover; beyond 32768 elements (16384 where rows are not
-// aligned: eight vectors spill there) the row is read twice.
+constexpr size_t kRowsRingBytes = 216 * 1024;  // rings of the streamed form
+
+// Streamed form: as many groups as the rings of two stages leave room for (32
+// at most; 15 where groups have several warps, and so a barrier each), more
+// stages where there is room.  A lane takes about eight vectors of a row, so
+// that the reduction is a small part of its work, but 15 warps are at work at
+// least.  Measured (us, bf16): 16384 elements, three groups of 5, 8, 10 warps
+// 50.9, 45.4, 49.1 (4992 rows); norm of 4608 with residual, five groups of 2,
+// 3, 4, 6 warps 403, 348, 372, 364 (65536 rows); 32768 elements, one group of
+// 12, 16, 24, 32 warps 167, 157, 169, 187 (8192 rows).  Rows that are not
+// aligned have many more instructions: all 32 warps (4607 elements, 1 or 2
+// warps a row: 270, 149).  Returns false where two stages of a row do not fit.
+bool plan_streamed_rows(Int8RowsParams* p, size_t slot, size_t code_bytes, size_t gain_bytes) {
+  if (gain_bytes >= kRowsRingBytes) return false;
+  const size_t room = kRowsRingBytes - gain_bytes;
+  const size_t stage = slot * (p->residual != nullptr ? 2 : 1);
+  int64_t groups = static_cast<int64_t>(room / (2 * stage + code_bytes));
+  if (groups < 1) return false;
+  if (groups > kRowsMaxGroups) groups = kRowsMaxGroups;
+  const int64_t vectors = ceil_div(p->cols, 8);
+  int64_t warps = 32 / groups;
+  if (code_bytes == 0) {
+    const int64_t enough = ceil_div(15, groups);
+    warps = (vectors + 128) / 256;
+    if (warps < enough) warps = enough;
+  }
+  if (warps > ceil_div(vectors, 32)) warps = ceil_div(vectors, 32);
+  if (warps < 1) warps = 1;
+  if (warps > 1 && groups > 15) groups = 15;
+  if (groups * warps > 32) groups = 32 / warps;
+  p->groups = static_cast<int32_t>(groups);
+  p->warps_per_row = static_cast<int32_t>(warps);
+  p->stages = kRowsMaxStages;
+  while (p->stages > 2 && groups * (p->stages * stage + code_bytes) > room) --p->stages;
+  return true;
+}
+
+template <class T, class G, bool kNorm, bool kVec>
+int launch_int8_rows_streamed(Int8RowsParams p, size_t shared, const DeviceInfo* info, cudaStream_t stream) {
+  static bool configured[kMaxDevices] = {};
+  p.timeout_ns = g_timeout_ns;
+  auto kernel = int8_rows_streamed_kernel<T, G, kNorm, kVec>;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  {
+    std::lock_guard<std::mutex> lock(g_device_mutex);
+    if (int rc = ensure_smem_attribute(configured[dev], kernel, kRowsRingBytes)) return rc;
+  }
+  const int64_t blocks = ceil_div(p.rows, p.groups);
+  const int sms = usable_sms(info);
+  const int grid = static_cast<int>(blocks < sms ? blocks : sms);
+  kernel<<<grid, 32 * p.warps_per_row * p.groups, shared, stream>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, kNorm ? "RMS norm (8-bit) launch" : "row quantisation launch");
+  return FMM_OK;
+}
+
+// Many rows are streamed.  Otherwise a row of up to 1024 elements is one
+// warp's (four vectors of 8 a lane), four rows a block; longer rows are a
+// block's, with the fewest vectors a thread that 1024 threads cover; beyond
+// 32768 elements the row is read twice.
 template <class T, class G, bool kNorm, bool kVec>
 int dispatch_int8_rows(Int8RowsParams p, const DeviceInfo* info, cudaStream_t stream) {
   const int64_t vectors = ceil_div(p.cols, 8);
+  const int64_t row_bytes = p.cols * int64_t(sizeof(T));
+  if (row_bytes >= 512 && (!kVec || row_bytes % 16 == 0)) {
+    const size_t slot = static_cast<size_t>(round_up(row_bytes, 16)) + (kVec ? 0 : 16);
+    const size_t code_bytes = kVec ? 0 : static_cast<size_t>(round_up(p.cols, 16));
+    Int8RowsParams streamed = p;
+    const size_t gain_bytes = kNorm ? static_cast<size_t>(round_up(p.cols * int64_t(4), 16)) : 0;
+    if (plan_streamed_rows(&streamed, slot, code_bytes, gain_bytes) &&
+        p.rows > 2 * int64_t(usable_sms(info)) * streamed.groups) {
+      const size_t shared =
+          gain_bytes + streamed.groups * (streamed.stages * slot * (p.residual != nullptr ? 2 : 1) + code_bytes);
+      return launch_int8_rows_streamed<T, G, kNorm, kVec>(streamed, shared, info, stream);
+    }
+  }
   if (vectors <= 128) {
     p.warps_per_row = 1;
     if (vectors <= 32) return launch_int8_rows<T, G, kNorm, 1, kVec>(p, 128, info, stream);
@@ -1041,12 +1112,6 @@ int dispatch_int8_rows(Int8RowsParams p, const DeviceInfo* info, cudaStream_t st
   if (warps(4) <= most) {
     p.warps_per_row = warps(4);
     return launch_int8_rows<T, G, kNorm, 4, kVec>(p, 32 * p.warps_per_row, info, stream);
-  }
-  if constexpr (kVec) {
-    if (warps(8) <= most) {
-      p.warps_per_row = warps(8);
-      return launch_int8_rows<T, G, kNorm, 8, kVec>(p, 32 * p.warps_per_row, info, stream);
-    }
   }
   p.warps_per_row = most;
   return launch_int8_rows<T, G, kNorm, 0, kVec>(p, kRowsMaxThreads, info, stream);

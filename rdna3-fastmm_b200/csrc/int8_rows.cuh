@@ -6,19 +6,24 @@
 //   a = max |p| over the row,  q = round_half_even(127 p / a)
 //
 // rstd cancels in q, so one reduction (sum of squares and maximum together)
-// separates the read of a row from its write: the row stays in registers and
-// every element crosses HBM once.
+// separates the read of a row from its write: a row stays on the chip in
+// between and every element crosses HBM once.
 //
 // Codes are those of exact arithmetic.  p is exact in FP32 where x and g have
-// 16 bits (at most 22 significant bits); with an FP32 gain it is the pair
-// hi + lo, lo = fma(h, g, -hi), and the maximum compares pairs.  p * (127 / a)
-// carries at most four roundings, 4 * 2^-24 * 127 < 2^-15, so only a quotient
-// within 2^-14 of a half can round the wrong way; those (1 in 8000) compare
-// 254 |p| with (2c + 1) a in FP64, where both products are exact.
+// 16 bits (at most 22 significant bits); with an FP32 gain the threads that
+// hold the largest rounded p look its FP64 value up.  127 / a is rounded, so
+// each product is taken by the FP32 numbers on either side of it; where the
+// two codes differ (1 product in 10^5), 254 p and (2c + 1) a are compared in
+// FP64, exact on both sides.
 //
 // A row with an infinity or a NaN (or, in the norm, with a square beyond FP32)
 // has codes 0 and a NaN scale: whatever is computed from it is NaN.  A row of
 // zeros has codes 0 and scale 0.
+//
+// Two kernels.  Few rows: a block (or a warp) a row, the row in registers, for
+// the shortest way from the first byte to the last.  Many rows: bound by HBM,
+// so rows arrive by bulk copies in a ring of shared memory and instructions are
+// counted (see int8_rows_streamed_kernel).
 #pragma once
 
 #include <type_traits>
@@ -27,7 +32,7 @@
 
 namespace fmm {
 
-constexpr int kRowsMaxThreads = 512;
+constexpr int kRowsMaxThreads = 1024;
 
 struct Int8RowsParams {
   const void* x;
@@ -40,7 +45,12 @@ struct Int8RowsParams {
   int64_t ldx, ldr, ldo, ldq;
   int32_t cols;
   float eps;
-  int32_t warps_per_row;  // > 1: the block is one row's; 1: every warp has a row of its own
+  // register form: > 1: the block is one row's; 1: every warp has a row of its own.
+  // Streamed form: the warps of a group
+  int32_t warps_per_row;
+  // streamed form: rows of a block at work, ring stages of each, and the waits' limit
+  int32_t groups, stages;
+  uint64_t timeout_ns;
 };
 
 // 8 consecutive elements as FP32, from a 16-byte aligned address (two for FP32).
@@ -89,82 +99,165 @@ struct RowVec<__half> {
   static __device__ __forceinline__ float wide(__half a) { return __half2float(a); }
 };
 
-// round_half_even(127 |P| / M) with the sign of P, for 0 <= |P| <= M, M > 0,
-// P and M of at most 44 significant bits: 254 |P| and (2c +- 1) M are exact.
-__device__ __forceinline__ int exact_code(double P, double M) {
-  const double a = 254.0 * fabs(P);
-  int c = static_cast<int>(floor((a / M + 1.0) * 0.5));
-  const double low = (2 * c - 1) * M, high = (2 * c + 1) * M;
-  if (a < low || (a == low && (c & 1))) --c;
-  else if (a > high || (a == high && (c & 1))) ++c;
-  return P < 0.0 ? -c : c;
+// round_half_even(127 P / M) where it is `below` or `below + 1`, M > 0, P and M
+// of at most 44 significant bits: both sides of the comparison are exact.
+__device__ __forceinline__ int exact_code(double P, double M, int below) {
+  const double value = 254.0 * P, border = (2 * below + 1) * M;
+  return value > border || (value == border && (below & 1)) ? below + 1 : below;
 }
 
-// What the row reduction gives: the sum of squares (norm only) and the
-// largest |p| as (bits of hi, lo).  Bits compare as the values do, infinities
-// and NaN above all finite ones.
+// The larger of m and |a|, |b|; NaN if one of them is.
+__device__ __forceinline__ float max_abs(float m, float a, float b) {
+  asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(a), "f"(b));
+  return m;
+}
+
+// What the row reduction gives: the sum of squares (norm only) and the bits of
+// the largest |p|, which compare as the values do, infinities and NaN above
+// all finite ones.
 struct RowTotals {
   float square;
-  uint32_t hi;
-  float lo;
+  uint32_t peak;
 };
 
-// Order-preserving map of a finite FP32 to unsigned, and back.
-__device__ __forceinline__ uint32_t float_key(float v) {
-  const uint32_t b = __float_as_uint(v);
-  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-}
-__device__ __forceinline__ float key_float(uint32_t k) {
-  return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
-}
-
-template <bool kNorm, bool kPair>
+template <bool kNorm>
 __device__ __forceinline__ RowTotals warp_totals(RowTotals t) {
-  RowTotals r = t;
   if constexpr (kNorm) {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) r.square += __shfl_xor_sync(0xffffffffu, r.square, d);
+    for (int d = 16; d > 0; d >>= 1) t.square += __shfl_xor_sync(0xffffffffu, t.square, d);
   }
-  r.hi = __reduce_max_sync(0xffffffffu, t.hi);
-  if constexpr (kPair)
-    r.lo = key_float(__reduce_max_sync(0xffffffffu, t.hi == r.hi ? float_key(t.lo) : 0u));
-  return r;
+  t.peak = __reduce_max_sync(0xffffffffu, t.peak);
+  return t;
 }
 
+// What a row's totals say about its codes.  A plain row multiplies by 127 / a,
+// computed from both sides: by `low` and by `high`, a few steps of FP32 apart
+// with the exact quotient between them.  Where both give the same code it is
+// the exact one; where they differ, the product is next to a border.  Rows that
+// are not plain (zeros, not finite, or so small or large that 127 / a leaves
+// FP32) take settled_code for every element, lifted into range.
+struct RowScale {
+  bool finite, zero;  // zero: all codes are 0
+  bool plain;
+  float lift;
+  float low, high;
+};
+// kPair: the product and the peak are rounded too
+template <bool kNorm, bool kPair>
+__device__ __forceinline__ RowScale row_scale(const RowTotals& total) {
+  RowScale s;
+  s.finite = total.peak < 0x7f800000u && (!kNorm || __float_as_uint(total.square) < 0x7f800000u);
+  s.zero = !s.finite || total.peak == 0u;
+  const float peak = __uint_as_float(total.peak);
+  s.plain = !s.zero && peak >= 0x1p-100f && peak <= 0x1p100f;
+  s.lift = peak < 0x1p-100f ? 0x1p100f : peak > 0x1p100f ? 0x1p-100f : 1.0f;
+  // the quotient is at most half a step off, the pair's other two roundings a step more each
+  constexpr uint32_t kSteps = kPair ? 3 : 1;
+  const uint32_t middle = __float_as_uint(127.0f / (s.zero ? 1.0f : peak * s.lift));
+  s.low = __uint_as_float(middle - kSteps);
+  s.high = __uint_as_float(middle + kSteps);
+  return s;
+}
+template <bool kNorm>
+__device__ __forceinline__ float stored_scale(const RowTotals& total, const RowScale& s, int cols, float eps) {
+  float scale = __uint_as_float(total.peak);
+  if constexpr (kNorm) scale = scale / sqrtf(total.square / static_cast<float>(cols) + eps);
+  return s.finite ? scale / 127.0f : __uint_as_float(0x7fc00000u);
+}
+
+// x + kMagic rounds x to an integer, the low byte of the sum: no conversions,
+// which run at an eighth of the rate.
+constexpr float kMagic = 0x1.8p23f;
+
+// Codes (low bytes) of 8 products of a plain row; the result has a bit set
+// where a product is next to a border.
+__device__ __forceinline__ uint32_t codes_of(const float (&p)[8], const RowScale& s, float (&code)[8],
+                                            float (&other)[8]) {
+  uint32_t differ = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    code[e] = fmaf(p[e], s.low, kMagic);
+    other[e] = fmaf(p[e], s.high, kMagic);
+    differ |= __float_as_uint(code[e]) ^ __float_as_uint(other[e]);
+  }
+  return differ;
+}
+__device__ __forceinline__ uint32_t border_mask(const float (&code)[8], const float (&other)[8]) {
+  uint32_t mask = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) mask |= code[e] != other[e] ? 1u << e : 0u;
+  return mask;
+}
+
+// Four codes: the low bytes of four words.
+__device__ __forceinline__ uint32_t pack_codes(float a, float b, float c, float d) {
+  const uint32_t low = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x0040);
+  const uint32_t high = __byte_perm(__float_as_uint(c), __float_as_uint(d), 0x0040);
+  return __byte_perm(low, high, 0x5410);
+}
+__device__ __forceinline__ uint2 pack_codes(const float (&code)[8]) {
+  return make_uint2(pack_codes(code[0], code[1], code[2], code[3]), pack_codes(code[4], code[5], code[6], code[7]));
+}
+
+// h + f rounded to the stream's type: the 8 elements as stored, and in h.
+template <class T>
+__device__ __forceinline__ uint4 add_vec(float (&h)[8], const float (&f)[8]) {
+  uint4 w;
+  w.x = RowVec<T>::pack(h[0] + f[0], h[1] + f[1]);
+  w.y = RowVec<T>::pack(h[2] + f[2], h[3] + f[3]);
+  w.z = RowVec<T>::pack(h[4] + f[4], h[5] + f[5]);
+  w.w = RowVec<T>::pack(h[6] + f[6], h[7] + f[7]);
+  RowVec<T>::load(reinterpret_cast<const T*>(&w), h);
+  return w;
+}
+
+// The code of a product next to a border or of a row that is not plain, P its
+// FP64 value.
+__device__ __forceinline__ int8_t settled_code(double P, double exact_peak, const RowScale& s) {
+  if (s.zero) return 0;
+  const double lifted = P * s.lift;
+  const int below = static_cast<int>(floorf(static_cast<float>(lifted) * s.low));
+  return static_cast<int8_t>(exact_code(lifted, exact_peak * s.lift, below));
+}
+
+// ---------------------------------------------------------------- few rows
 // V: vectors of 8 elements a thread holds in registers (0: the row is read
 // twice in a loop, for rows beyond the registers of a block).  kVec: rows of
 // every tensor start on 16-byte boundaries (8 for the codes), a thread's 8
 // elements are consecutive; otherwise they are a block's width apart, so that
 // 2-byte and 4-byte accesses still coalesce.
 template <class T, class G, bool kNorm, int V, bool kVec>
-__global__ void __launch_bounds__(kRowsMaxThreads) int8_rows_kernel(const Int8RowsParams p) {
+__global__ void __launch_bounds__(kRowsMaxThreads, 1) int8_rows_kernel(const Int8RowsParams p) {
   constexpr bool kPair = kNorm && std::is_same<G, float>::value;
   constexpr int kHeld = V > 0 ? V : 1;
   __shared__ float s_square[2][32];
-  __shared__ uint32_t s_hi[2][32];
-  __shared__ float s_lo[2][32];
+  __shared__ uint32_t s_peak[2][32];
+  __shared__ unsigned long long s_exact[2];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const bool block_row = p.warps_per_row > 1;
   const int rows_per_block = block_row ? 1 : blockDim.x / 32;
-  const int width = block_row ? blockDim.x : 32;           // threads of a row
+  const int width = block_row ? blockDim.x : 32;  // threads of a row
   const int t = block_row ? threadIdx.x : lane;
   const int cols = p.cols;
+  const bool add = kNorm && p.residual != nullptr;
   const G* gain = static_cast<const G*>(p.gain);
   // first element of this thread's vector v, and the step between its elements
   const int step = kVec ? 1 : width;
   auto first = [&](int v) { return kVec ? (v * width + t) * 8 : v * 8 * width + t; };
   const int loops = V > 0 ? V : (cols + 8 * width - 1) / (8 * width);
+  if (kPair && threadIdx.x < 2) s_exact[threadIdx.x] = 0;
 
   int parity = 0;
   for (int64_t row = int64_t(blockIdx.x) * rows_per_block + (block_row ? 0 : warp); row < p.rows;
        row += int64_t(gridDim.x) * rows_per_block) {
     const T* x = static_cast<const T*>(p.x) + row * p.ldx;
-    const T* r = (kNorm && p.residual != nullptr) ? static_cast<const T*>(p.residual) + row * p.ldr : nullptr;
-    T* ro = r != nullptr ? static_cast<T*>(p.residual_out) + row * p.ldo : nullptr;
+    const T* r = add ? static_cast<const T*>(p.residual) + row * p.ldr : nullptr;
+    T* ro = add ? static_cast<T*>(p.residual_out) + row * p.ldo : nullptr;
+    const T* stream = add ? ro : x;  // h in memory, once this thread has read its elements
     int8_t* q = p.codes + row * p.ldq;
 
     // h of vector v: x, or x + r rounded to the stream's type; past the end 0
-    auto read = [&](int v, const T* a, const T* b, T* out, float (&h)[8]) {
+    auto read = [&](int v, const T* a, const T* b, float (&h)[8]) {
       const int c0 = first(v);
       if (kVec && c0 + 8 <= cols) {
         RowVec<T>::load(a + c0, h);
@@ -172,13 +265,7 @@ __global__ void __launch_bounds__(kRowsMaxThreads) int8_rows_kernel(const Int8Ro
           if (b != nullptr) {
             float f[8];
             RowVec<T>::load(b + c0, f);
-            uint4 w;
-            w.x = RowVec<T>::pack(h[0] + f[0], h[1] + f[1]);
-            w.y = RowVec<T>::pack(h[2] + f[2], h[3] + f[3]);
-            w.z = RowVec<T>::pack(h[4] + f[4], h[5] + f[5]);
-            w.w = RowVec<T>::pack(h[6] + f[6], h[7] + f[7]);
-            *reinterpret_cast<uint4*>(out + c0) = w;
-            RowVec<T>::load(reinterpret_cast<const T*>(&w), h);
+            *reinterpret_cast<uint4*>(ro + c0) = add_vec<T>(h, f);
           }
         }
         return;
@@ -192,128 +279,477 @@ __global__ void __launch_bounds__(kRowsMaxThreads) int8_rows_kernel(const Int8Ro
           if constexpr (kNorm) {
             if (b != nullptr) {
               const T s = RowVec<T>::rnd(h[e] + RowVec<T>::one(b + c));
-              out[c] = s;
+              ro[c] = s;
               h[e] = RowVec<T>::wide(s);
             }
           }
         }
       }
     };
-    auto read_gain = [&](int v, float (&g)[8]) {
-      const int c0 = first(v);
-      if (kVec && c0 + 8 <= cols) {
-        RowVec<G>::load(gain + c0, g);
-        return;
-      }
+    // h -> p in place
+    auto times_gain = [&](int v, float (&h)[8]) {
+      if constexpr (kNorm) {
+        const int c0 = first(v);
+        float g[8];
+        if (kVec && c0 + 8 <= cols) {
+          RowVec<G>::load(gain + c0, g);
+        } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) g[e] = c0 + e * step < cols ? RowVec<G>::one(gain + c0 + e * step) : 0.0f;
+          for (int e = 0; e < 8; ++e) g[e] = c0 + e * step < cols ? RowVec<G>::one(gain + c0 + e * step) : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] *= g[e];
+      }
     };
-    // h -> p in place, taking part in the totals
-    auto take = [&](int v, float (&h)[8], RowTotals& total) {
-      float g[8];
-      if constexpr (kNorm) read_gain(v, g);
+    float square = 0.0f, most = 0.0f;
+    auto take = [&](int v, float (&h)[8]) {
+      if constexpr (kNorm) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float was = h[e];
-        if constexpr (kNorm) {
-          total.square = fmaf(was, was, total.square);
-          h[e] = was * g[e];
-        }
-        const uint32_t hi = __float_as_uint(fabsf(h[e]));
-        if constexpr (kPair) {
-          const float rest = fmaf(was, g[e], -h[e]);
-          const float lo = h[e] < 0.0f ? -rest : rest;
-          if (hi > total.hi || (hi == total.hi && lo > total.lo)) total.lo = lo;
-        }
-        total.hi = max(total.hi, hi);
+        for (int e = 0; e < 8; ++e) square = fmaf(h[e], h[e], square);
       }
+      times_gain(v, h);
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) most = max_abs(most, h[e], h[e + 1]);
+    };
+    // p of one element in FP64, exact, from memory
+    auto exact = [&](int c) {
+      double P = static_cast<double>(RowVec<T>::one(stream + c));
+      if constexpr (kNorm) P *= static_cast<double>(RowVec<G>::one(gain + c));
+      return P;
     };
 
     float held[kHeld][8];
-    RowTotals total = {0.0f, 0u, 0.0f};
     if constexpr (V > 0) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) read(v, x, r, ro, held[v]);
+      for (int v = 0; v < V; ++v) read(v, x, r, held[v]);
 #pragma unroll
-      for (int v = 0; v < V; ++v) take(v, held[v], total);
+      for (int v = 0; v < V; ++v) take(v, held[v]);
     } else {
       for (int v = 0; v < loops; ++v) {
-        read(v, x, r, ro, held[0]);
-        take(v, held[0], total);
+        read(v, x, r, held[0]);
+        take(v, held[0]);
       }
     }
-    total = warp_totals<kNorm, kPair>(total);
+    const uint32_t mine = __float_as_uint(most);
+    RowTotals total = warp_totals<kNorm>({square, mine});
     if (block_row) {
       if (lane == 0) {
         s_square[parity][warp] = total.square;
-        s_hi[parity][warp] = total.hi;
-        s_lo[parity][warp] = total.lo;
+        s_peak[parity][warp] = total.peak;
       }
       // one barrier a row: the other half of the arrays is written next
       __syncthreads();
       const bool in = lane < p.warps_per_row;
       total.square = in ? s_square[parity][lane] : 0.0f;
-      total.hi = in ? s_hi[parity][lane] : 0u;
-      total.lo = in ? s_lo[parity][lane] : 0.0f;
-      total = warp_totals<kNorm, kPair>(total);
-      parity ^= 1;
+      total.peak = in ? s_peak[parity][lane] : 0u;
+      total = warp_totals<kNorm>(total);
     }
-
-    const float peak = __uint_as_float(total.hi);
-    bool finite = total.hi < 0x7f800000u;
-    float scale = peak;
-    if constexpr (kNorm) {
-      const float mean = total.square / static_cast<float>(cols);
-      finite = finite && __float_as_uint(mean) < 0x7f800000u;
-      scale = peak / sqrtf(mean + p.eps);
+    const RowScale scale = row_scale<kNorm, kPair>(total);
+    if (t == 0) p.scales[row] = stored_scale<kNorm>(total, scale, cols, p.eps);
+    double exact_peak = __uint_as_float(total.peak);
+    if constexpr (kPair) {
+      // p is rounded here: those who hold the largest look it up in FP64
+      unsigned long long bits = 0;
+      if (mine == total.peak && scale.finite) {
+        double value = 0.0;
+        if constexpr (V > 0) {
+          uint32_t largest = 0;
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              largest |= __float_as_uint(fabsf(held[v][e])) == total.peak ? 1u << (8 * v + e) : 0u;
+#pragma unroll 1
+          for (; largest != 0; largest &= largest - 1) {
+            const int i = __ffs(largest) - 1, c = first(i >> 3) + (i & 7) * step;
+            if (c < cols) value = fmax(value, fabs(exact(c)));
+          }
+        } else {
+          for (int v = 0; v < loops; ++v)
+            for (int c = first(v); c < min(first(v) + 8 * step, cols); c += step) value = fmax(value, fabs(exact(c)));
+        }
+        bits = static_cast<unsigned long long>(__double_as_longlong(value));
+      }
+      if (block_row) {
+        if (bits != 0) atomicMax(&s_exact[parity], bits);
+        if (threadIdx.x == 0) s_exact[parity ^ 1] = 0;  // nobody reads it before the next row's first barrier
+        __syncthreads();
+        bits = s_exact[parity];
+      } else {
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, d));
+      }
+      exact_peak = __longlong_as_double(static_cast<long long>(bits));
     }
-    scale = finite ? scale / 127.0f : __uint_as_float(0x7fc00000u);
-    if (t == 0) p.scales[row] = scale;
-    const bool zero = !finite || total.hi == 0u;
-    // 127 / peak leaves FP32 below 2^-121; such rows take the exact codes
-    const bool tiny = peak < 0x1p-100f;
-    const float inverse = zero || tiny ? 0.0f : 127.0f / peak;
-    const double exact_peak = static_cast<double>(peak) + (kPair ? static_cast<double>(total.lo) : 0.0);
+    parity ^= 1;
 
 #pragma unroll
     for (int v = 0; v < loops; ++v) {
       const int c0 = first(v);
       if (V == 0) {
         // second reading: the stream as stored, or x
-        RowTotals unused = {0.0f, 0u, 0.0f};
-        read(v, ro != nullptr ? ro : x, nullptr, nullptr, held[0]);
-        take(v, held[0], unused);
+        read(v, stream, nullptr, held[0]);
+        times_gain(v, held[0]);
       }
-      float(&pv)[8] = held[V > 0 ? v : 0];
-      int code[8];
-      bool border = tiny && !zero;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float d = zero ? 0.0f : pv[e] * inverse;
-        code[e] = __float2int_rn(d);
-        border = border || fabsf(d - static_cast<float>(code[e])) > 0.5f - 0x1p-14f;
+      if (!scale.plain) {
+        for (int c = c0; c < min(c0 + 8 * step, cols); c += step)
+          q[c] = settled_code(scale.zero ? 0.0 : exact(c), exact_peak, scale);
+        continue;
       }
+      float code[8], other[8];
+      const uint32_t differ = codes_of(held[V > 0 ? v : 0], scale, code, other);
       if (kVec && c0 + 8 <= cols) {
-        uint2 w;
-        w.x = (code[0] & 255) | (code[1] & 255) << 8 | (code[2] & 255) << 16 | code[3] << 24;
-        w.y = (code[4] & 255) | (code[5] & 255) << 8 | (code[6] & 255) << 16 | code[7] << 24;
-        *reinterpret_cast<uint2*>(q + c0) = w;
+        *reinterpret_cast<uint2*>(q + c0) = pack_codes(code);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (c0 + e * step < cols) q[c0 + e * step] = static_cast<int8_t>(code[e]);
+          if (c0 + e * step < cols) q[c0 + e * step] = static_cast<int8_t>(__float_as_uint(code[e]));
       }
-      if (border) {
-        // once more from memory (this thread's own elements), in FP64
-        const T* h = ro != nullptr ? ro : x;
+      if (differ != 0) {
+        uint32_t near = border_mask(code, other);
 #pragma unroll 1
-        for (int c = c0; c < min(c0 + 8 * step, cols); c += step) {
-          double P = static_cast<double>(RowVec<T>::one(h + c));
-          if constexpr (kNorm) P *= static_cast<double>(RowVec<G>::one(gain + c));
-          q[c] = static_cast<int8_t>(exact_code(P, exact_peak));
+        for (; near != 0; near &= near - 1) {
+          const int c = c0 + (__ffs(near) - 1) * step;
+          if (c < cols) q[c] = settled_code(exact(c), exact_peak, scale);
         }
       }
     }
+  }
+}
+
+// ---------------------------------------------------------------- many rows
+// Bulk copy of 16-byte units (both addresses aligned) into this CTA's shared
+// memory, completing on the mbarrier at `bar`.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+      : "memory");
+}
+
+// The 16-byte units of a row: `count` elements from element `head` on.
+struct RowBody {
+  int head, count;
+};
+template <class T>
+__device__ __forceinline__ RowBody row_body(const T* row, int cols) {
+  constexpr int kUnit = 16 / sizeof(T);
+  const int off = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
+  const int head = min((kUnit - off) & (kUnit - 1), cols);
+  return {head, (cols - head) & ~(kUnit - 1)};
+}
+
+constexpr int kRowsMaxGroups = 32;
+constexpr int kRowsMaxStages = 4;
+
+// One CTA an SM; `groups` groups of `warps_per_row` warps, each with rows of
+// its own and a ring of `stages` rows of shared memory that bulk copies fill,
+// so HBM is busy while rows are reduced and converted.  A row is read from its
+// stage twice (totals, then codes): nothing is held in registers, few warps
+// share a row (a reduction costs each of them some 100 instructions whatever
+// the row's length), and groups wait for nobody but their own warps.  With a
+// residual the sum goes back into the stage, and to memory; the gain has an FP32
+// copy in shared memory.
+//
+// kVec: rows and leading dimensions are whole 16-byte units.  Otherwise copies
+// move the whole units inside a row and the few elements at its ends are put
+// into the stage by threads; accesses are one element wide, `width` threads
+// apart, and codes are collected in shared memory.
+template <class T, class G, bool kNorm, bool kVec>
+__global__ void __launch_bounds__(kRowsMaxThreads, 1) int8_rows_streamed_kernel(const Int8RowsParams p) {
+  constexpr bool kPair = kNorm && std::is_same<G, float>::value;
+  __shared__ __align__(8) uint64_t s_full[kRowsMaxGroups * kRowsMaxStages];
+  __shared__ float s_square[kRowsMaxGroups];
+  __shared__ uint32_t s_peak[kRowsMaxGroups];
+  __shared__ unsigned long long s_exact[kRowsMaxGroups];
+  __shared__ int s_abort[kRowsMaxGroups];
+  extern __shared__ __align__(128) uint8_t s_ring[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int warps = p.warps_per_row, width = warps * 32;
+  const int group = warp / warps, t = threadIdx.x - group * width;
+  const int cols = p.cols;
+  const bool add = kNorm && p.residual != nullptr;
+  float* gain = reinterpret_cast<float*>(s_ring);
+  const uint32_t gain_bytes = kNorm ? (static_cast<uint32_t>(cols) * 4u + 15u) / 16u * 16u : 0u;
+  const uint32_t slot = (static_cast<uint32_t>(cols) * sizeof(T) + 15u) / 16u * 16u + (kVec ? 0u : 16u);
+  const uint32_t stage_bytes = slot * (add ? 2u : 1u);
+  const uint32_t code_bytes = kVec ? 0u : (static_cast<uint32_t>(cols) + 15u) / 16u * 16u;
+  uint8_t* ring = s_ring + gain_bytes + static_cast<size_t>(group) * (p.stages * stage_bytes + code_bytes);
+  int8_t* s_codes = reinterpret_cast<int8_t*>(ring + p.stages * stage_bytes);
+  const uint32_t full_bar = smem_u32(s_full + group * kRowsMaxStages);
+  // consecutive rows go to consecutive SMs, so that SMs differ by a row at most
+  const int64_t row0 = int64_t(group) * gridDim.x + blockIdx.x, row_step = int64_t(gridDim.x) * p.groups;
+  // kVec: the first halves of the gain's vectors, then the second halves, so
+  // that lanes read 16 bytes apart (32 apart, two of them share a bank)
+  auto gain_at = [&](int c) { return kVec ? gain[((c & 4) ? cols / 2 : 0) + c / 8 * 4 + (c & 3)] : gain[c]; };
+  auto load_gain = [&](int c, float (&g)[8]) {
+    const float4 a = *reinterpret_cast<const float4*>(gain + c / 2);
+    const float4 b = *reinterpret_cast<const float4*>(gain + (cols + c) / 2);
+    g[0] = a.x; g[1] = a.y; g[2] = a.z; g[3] = a.w;
+    g[4] = b.x; g[5] = b.y; g[6] = b.z; g[7] = b.w;
+  };
+  auto group_sync = [&] {
+    if (warps == 1) __syncwarp();
+    else named_barrier_sync(1 + group, width);
+  };
+  // where element 0 of a row is in its slot: bodies start on 16-byte boundaries
+  auto origin = [&](const T* row) { return kVec ? 0u : static_cast<uint32_t>(reinterpret_cast<uintptr_t>(row) & 15u); };
+  // thread 0 of the group: fetch `row` into `stage`
+  auto fetch = [&](int64_t row, int stage) {
+    const uint32_t bar = full_bar + 8 * stage, dst = smem_u32(ring + stage * stage_bytes);
+    const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+    const T* r = add ? static_cast<const T*>(p.residual) + row * p.ldr : nullptr;
+    const RowBody a = kVec ? RowBody{0, cols} : row_body(x, cols);
+    const RowBody b = !add ? RowBody{0, 0} : kVec ? RowBody{0, cols} : row_body(r, cols);
+    mbar_arrive_expect_tx(bar, static_cast<uint32_t>((a.count + b.count) * sizeof(T)));
+    if (a.count > 0) bulk_load(dst + origin(x) + a.head * sizeof(T), x + a.head, a.count * sizeof(T), bar);
+    if (b.count > 0) bulk_load(dst + slot + origin(r) + b.head * sizeof(T), r + b.head, b.count * sizeof(T), bar);
+  };
+  if (t == 0) {
+    s_abort[group] = 0;
+    for (int s = 0; s < p.stages; ++s) mbar_init(full_bar + 8 * s, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    for (int s = 0; s < p.stages; ++s)
+      if (row0 + s * row_step < p.rows) fetch(row0 + s * row_step, s);
+  }
+  if (threadIdx.x < kRowsMaxGroups) s_exact[threadIdx.x] = 0;
+  if constexpr (kNorm) {
+    const G* source = static_cast<const G*>(p.gain);
+    if constexpr (kVec) {
+      for (int c = 8 * threadIdx.x; c < cols; c += 8 * blockDim.x) {
+        float g[8];
+        RowVec<G>::load(source + c, g);
+        *reinterpret_cast<float4*>(gain + c / 2) = make_float4(g[0], g[1], g[2], g[3]);
+        *reinterpret_cast<float4*>(gain + (cols + c) / 2) = make_float4(g[4], g[5], g[6], g[7]);
+      }
+    } else {
+      for (int c = threadIdx.x; c < cols; c += blockDim.x) gain[c] = RowVec<G>::one(source + c);
+    }
+  }
+  __syncthreads();
+
+  int stage = 0;
+  uint32_t phase = 0;
+  for (int64_t row = row0; row < p.rows; row += row_step) {
+    int8_t* q = p.codes + row * p.ldq;
+    T* ro = add ? static_cast<T*>(p.residual_out) + row * p.ldo : nullptr;
+    // a wait that runs out is noticed by the whole group behind its barrier
+    mbar_wait_bounded(full_bar + 8 * stage, phase, &s_abort[group], p.timeout_ns, 31);
+    uint8_t* bytes = ring + stage * stage_bytes;
+    T* h = reinterpret_cast<T*>(bytes);
+    const T* f = reinterpret_cast<const T*>(bytes + slot);
+    if constexpr (!kVec) {
+      const T* x = static_cast<const T*>(p.x) + row * p.ldx;
+      const RowBody a = row_body(x, cols);
+      h = reinterpret_cast<T*>(bytes + origin(x));
+      // what the copies leave out: fewer than 16 elements at each end
+      for (int c = t; c < cols - a.count; c += width) {
+        const int at = c < a.head ? c : c + a.count;
+        h[at] = x[at];
+      }
+      if (add) {
+        const T* r = static_cast<const T*>(p.residual) + row * p.ldr;
+        const RowBody b = row_body(r, cols);
+        T* left = reinterpret_cast<T*>(bytes + slot + origin(r));
+        for (int c = t; c < cols - b.count; c += width) {
+          const int at = c < b.head ? c : c + b.count;
+          left[at] = r[at];
+        }
+        f = left;
+      }
+      group_sync();
+    }
+
+    // ---- totals
+    float square = 0.0f, square_b = 0.0f, most = 0.0f;
+    // FP32 gain: where this thread's largest product was, and whether a later
+    // vector had one as large
+    int at = 0;
+    bool again = false;
+    auto take = [&](float largest, int c) {
+      if constexpr (kPair) {
+        again = largest > most ? false : again || largest == most;
+        at = largest > most ? c : at;
+      }
+      most = max_abs(most, largest, largest);
+    };
+    if constexpr (kVec) {
+#pragma unroll 4
+      for (int c = 8 * t; c < cols; c += 8 * width) {
+        float v[8];
+        RowVec<T>::load(h + c, v);
+        if constexpr (kNorm) {
+          if (add) {
+            float w[8];
+            RowVec<T>::load(f + c, w);
+            const uint4 sum = add_vec<T>(v, w);
+            *reinterpret_cast<uint4*>(h + c) = sum;
+            *reinterpret_cast<uint4*>(ro + c) = sum;
+          }
+          float g[8];
+          load_gain(c, g);
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            square = fmaf(v[e], v[e], square);
+            square_b = fmaf(v[e + 1], v[e + 1], square_b);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= g[e];
+        }
+        if constexpr (kPair) {
+          float largest = 0.0f;
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) largest = max_abs(largest, v[e], v[e + 1]);
+          take(largest, c);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) most = max_abs(most, v[e], v[e + 1]);
+        }
+      }
+    } else {
+#pragma unroll 4
+      for (int c = t; c < cols; c += width) {
+        float v = RowVec<T>::one(h + c);
+        if constexpr (kNorm) {
+          if (add) {
+            const T s = RowVec<T>::rnd(v + RowVec<T>::one(f + c));
+            h[c] = s;
+            ro[c] = s;
+            v = RowVec<T>::wide(s);
+          }
+          square = fmaf(v, v, square);
+          v *= gain[c];
+        }
+        take(fabsf(v), c);
+      }
+    }
+    const uint32_t mine = __float_as_uint(most);
+    RowTotals total = warp_totals<kNorm>({square + square_b, mine});
+    if (warps > 1) {
+      if (lane == 0) {
+        s_square[warp] = total.square;
+        s_peak[warp] = total.peak;
+      }
+      group_sync();
+      total.square = 0.0f;
+      total.peak = 0u;
+      for (int w = group * warps; w < (group + 1) * warps; ++w) {
+        total.square += s_square[w];
+        total.peak = max(total.peak, s_peak[w]);
+      }
+    }
+    if (warps == 1 ? __any_sync(0xffffffffu, *static_cast<volatile int*>(&s_abort[group]) != 0)
+                   : *static_cast<volatile int*>(&s_abort[group]) != 0)
+      break;
+    const RowScale scale = row_scale<kNorm, kPair>(total);
+    if (t == 0) p.scales[row] = stored_scale<kNorm>(total, scale, cols, p.eps);
+    // p of one element in FP64, exact
+    auto exact = [&](int c) {
+      double P = static_cast<double>(RowVec<T>::one(h + c));
+      if constexpr (kNorm) P *= static_cast<double>(gain_at(c));
+      return P;
+    };
+    double exact_peak = __uint_as_float(total.peak);
+    if constexpr (kPair) {
+      // p is rounded here: those who hold the largest look it up in FP64
+      unsigned long long bits = 0;
+      if (mine == total.peak && !scale.zero) {
+        double value = 0.0;
+        auto look = [&](int c0) {
+#pragma unroll
+          for (int e = 0; e < (kVec ? 8 : 1); ++e) {
+            const float a = RowVec<T>::one(h + c0 + e), g = gain_at(c0 + e);
+            if (__float_as_uint(fabsf(a * g)) == total.peak)
+              value = fmax(value, fabs(static_cast<double>(a) * static_cast<double>(g)));
+          }
+        };
+        if (!again) {
+          look(at);
+        } else {
+          const int step = kVec ? 8 : 1;
+          for (int c = step * t; c < cols; c += step * width) look(c);
+        }
+        bits = static_cast<unsigned long long>(__double_as_longlong(value));
+      }
+      if (warps > 1) {
+        if (bits != 0) atomicMax(&s_exact[group], bits);
+        group_sync();
+        bits = s_exact[group];
+      } else {
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, d));
+      }
+      exact_peak = __longlong_as_double(static_cast<long long>(bits));
+    }
+
+    // ---- codes
+    if (!scale.plain) {
+      for (int c = t; c < cols; c += width) {
+        const int8_t byte = settled_code(scale.zero ? 0.0 : exact(c), exact_peak, scale);
+        if constexpr (kVec) q[c] = byte;
+        else s_codes[c] = byte;
+      }
+    } else if constexpr (kVec) {
+#pragma unroll 4
+      for (int c = 8 * t; c < cols; c += 8 * width) {
+        float v[8];
+        RowVec<T>::load(h + c, v);
+        if constexpr (kNorm) {
+          float g[8];
+          load_gain(c, g);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= g[e];
+        }
+        float code[8], other[8];
+        const uint32_t differ = codes_of(v, scale, code, other);
+        *reinterpret_cast<uint2*>(q + c) = pack_codes(code);
+        if (differ != 0) {
+          uint32_t near = border_mask(code, other);
+#pragma unroll 1
+          for (; near != 0; near &= near - 1) {
+            const int at = c + __ffs(near) - 1;
+            q[at] = settled_code(exact(at), exact_peak, scale);
+          }
+        }
+      }
+    } else {
+#pragma unroll 4
+      for (int c = t; c < cols; c += width) {
+        float v = RowVec<T>::one(h + c);
+        if constexpr (kNorm) v *= gain[c];
+        const float code = fmaf(v, scale.low, kMagic);
+        int8_t byte = static_cast<int8_t>(__float_as_uint(code));
+        if (code != fmaf(v, scale.high, kMagic)) byte = settled_code(exact(c), exact_peak, scale);
+        s_codes[c] = byte;
+      }
+    }
+    // this thread's writes to the stage come before the copy that refills it
+    if (add || !kVec) fence_proxy_async_smem();
+    group_sync();
+    if (t == 0) {
+      if (kPair) s_exact[group] = 0;  // read by all; the next row's first barrier comes before its use
+      if (row + p.stages * row_step < p.rows) fetch(row + p.stages * row_step, stage);
+    }
+    if constexpr (!kVec) {
+      // collected codes, 16 at a time where the row allows it; the next row
+      // writes them behind a barrier that follows
+      const bool whole = (reinterpret_cast<uintptr_t>(q) & 15u) == 0;
+      const int units = whole ? cols / 16 : 0;
+      for (int u = t; u < units; u += width)
+        *reinterpret_cast<uint4*>(q + 16 * u) = *reinterpret_cast<const uint4*>(s_codes + 16 * u);
+      for (int c = 16 * units + t; c < cols; c += width) q[c] = s_codes[c];
+    }
+    if (++stage == p.stages) {
+      stage = 0;
+      phase ^= 1u;
+    }
+  }
+  if (s_abort[group] != 0 && t == 0) {
+    // copies into this group's ring may still be landing: give each its limit
+    volatile int no_abort = 0;
+    for (int s = 0; s < p.stages; ++s)
+      if (row0 + s * row_step < p.rows)
+        mbar_wait_bounded(full_bar + 8 * s, s < stage ? phase ^ 1u : phase, &no_abort, p.timeout_ns, 32);
   }
 }
 

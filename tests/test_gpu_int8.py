@@ -62,7 +62,7 @@ def _norm_roundings(inner):
     # ten halvings join a block; the root halves what the mean is off, four
     # roundings follow (mean + eps counts in the sum; root, two quotients, peak)
     vectors = -(-inner // 8)
-    mine = 8 * max(-(-vectors // 512), 4)
+    mine = 8 * max(-(-vectors // 1024), 4)
     return (mine + 12) / 2 + 4
 
 
@@ -130,6 +130,32 @@ def test_rows_of_zeros_infinities_and_nans(inner):
                         scales.to(DEVICE), wc, ws).cpu()
         assert not y[1].any()
         assert y[2:4].isnan().all()
+
+
+@pytest.mark.parametrize("with_residual", [False, True])
+@pytest.mark.parametrize("gain", ["same", "fp32"])
+@pytest.mark.parametrize("rows,inner", [(12001, 512), (11003, 1024), (4097, 1032), (1201, 4608), (700, 8200), (401, 16384),
+                                        (330, 24576), (310, 32768), (333, 4607)])
+def test_many_rows_stream_through(rows, inner, gain, with_residual):
+    """More rows than resident blocks take at once; padding rows among them."""
+    x = _randn((rows, inner), 1, BF16).to(DEVICE)
+    x[rows // 2:rows // 2 + 40] = 0
+    residual = _randn((rows, inner), 2, BF16).to(DEVICE) if with_residual else None
+    if with_residual:
+        residual[rows // 2:rows // 2 + 40] = 0
+    weight = (1 + 0.3 * _randn((inner,), 3)).to(FP32 if gain == "fp32" else BF16).to(DEVICE)
+    codes, scales, stream = rms_norm_int8(x, weight, residual, 1e-5)
+    h, p, rstd = _norm_reference(x, weight, residual, 1e-5)
+    expected, peak = _codes(p)
+    assert torch.equal(codes, expected.to(torch.int8))
+    reference = peak * rstd / 127.0
+    assert bool(((scales.double() - reference).abs() <= _norm_roundings(inner) * U32 * reference).all())
+    if with_residual:
+        assert torch.equal(stream, h)
+    codes, scales = quantize_rows(x)
+    expected, peak = _codes(x.double())
+    assert torch.equal(codes, expected.to(torch.int8))
+    assert bool(((scales.double() - peak / 127.0).abs() <= U32 * peak / 127.0).all())
 
 
 @pytest.mark.parametrize("scale", [2.0**-130, 2.0**-110, 2.0**100])
