@@ -1156,42 +1156,219 @@ int codes_map(CUtensorMap* map, const void* base, int64_t k, int64_t rows, int64
 
 constexpr size_t kI8MaxSmem = 232448;
 
+// How int8_linear_kernel takes a product: channels and tokens of a tile.
+struct Int8Shape {
+  int rows, tok;
+};
+
+// Measured (one B200, us a 128-deep column of K): a tile of 128 channels costs
+// 0.15 + 0.0011 tok (tok = 64, 128, 192, 256: 0.20, 0.28, 0.36, 0.43), one of 64
+// channels about an eighth less, a 256 x 256 tile of two SMs 0.37 however
+// many of its tokens exist; every launch some 4 more.  The estimates pick the
+// least whole waves of tiles.
+double int8_single_cost(int64_t M, int64_t K, int64_t N, const Int8Shape& s, int sms) {
+  const int64_t tiles = ceil_div(M, s.tok) * ceil_div(N, s.rows);
+  const double column = (0.15 + 0.0011 * s.tok) * (s.rows < kI8TileN ? 0.875 : 1.0);
+  return 4.0 + double(ceil_div(tiles, sms)) * double(ceil_div(K, kI8BlockK)) * column;
+}
+double int8_pair_cost(int64_t M, int64_t K, int64_t N, int sms) {
+  const int64_t tiles = ceil_div(M, 256) * ceil_div(N, 256);
+  return 5.0 + double(ceil_div(tiles, sms / 2)) * double(ceil_div(K, kI8BlockK)) * 0.37;
+}
+
+Int8Shape choose_int8_shape(int64_t M, int64_t K, int64_t N, int sms, double* cost) {
+  Int8Shape best = {kI8TileN, 16};
+  *cost = 1e30;
+  auto consider = [&](int64_t tok) {
+    for (int rows : {kI8TileN, kI8TileN / 2}) {
+      const Int8Shape s = {rows, static_cast<int>(tok)};
+      const double c = int8_single_cost(M, K, N, s, sms);
+      if (c < *cost) {
+        *cost = c;
+        best = s;
+      }
+    }
+  };
+  // the tokens in equal tiles, and the widths that tiles of many tokens have
+  for (int64_t pieces = ceil_div(M, 256); pieces <= 16; ++pieces) consider(round_up(ceil_div(M, pieces), 16));
+  if (M > 256)
+    for (int64_t tok : {64, 96, 128, 192, 256}) consider(tok);
+  return best;
+}
+
 template <bool kBf16>
-int launch_linear_int8(const int8_t* codes, int64_t ldq, const int8_t* weight_codes, int64_t ldw,
-                       Int8LinearParams p, cudaStream_t stream) {
+int launch_int8_single(const int8_t* codes, int64_t ldq, const int8_t* weight_codes, int64_t ldw, Int8LinearParams p,
+                       const Int8Shape& shape, int sms, cudaStream_t stream) {
   static bool configured[kMaxDevices] = {};
-  DeviceInfo* info = nullptr;
-  if (int rc = device_info(&info)) return rc;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
-  p.tok = static_cast<int32_t>(p.M >= 256 ? 256 : round_up(p.M, 16));
+  p.rows = shape.rows;
+  p.tok = shape.tok;
   p.tmem_cols = 32;
   while (p.tmem_cols < static_cast<uint32_t>(p.tok)) p.tmem_cols *= 2;
-  const int64_t tiles_m = ceil_div(p.M, p.tok), tiles_n = ceil_div(p.N, kI8TileN);
-  if (tiles_m * tiles_n > (int64_t(1) << 30)) return fail(FMM_ERR_TOO_LARGE, "too many tiles");
-  p.tiles_m = static_cast<int32_t>(tiles_m);
-  p.tiles_n = static_cast<int32_t>(tiles_n);
-  const size_t stage = kI8WBytes + size_t(p.tok) * kI8BlockK;
-  const size_t control = 1024 + 8 * (2 * kI8MaxStages + 4);
+  p.tiles_m = static_cast<int32_t>(ceil_div(p.M, p.tok));
+  p.tiles_n = static_cast<int32_t>(ceil_div(p.N, p.rows));
+  // 128-deep columns of a stage: as many as keep it at 64 KB (three stages), up
+  // to four.  64 channels x 16 tokens, K = 4096, with 1, 2, 4: 13.4, 10.7, 10.0
+  // us; 128 x 128: 14.3, 13.5; 128 x 192 with 1, 2: 27.1, 32.8
+  p.atoms = p.rows + p.tok <= 128 ? 4 : p.rows + p.tok <= 256 ? 2 : 1;
+  const size_t stage = p.atoms * size_t(p.rows + p.tok) * kI8BlockK;
+  // alignment, barriers, and the rows that products read behind the last stage's
+  const size_t control = 1024 + 8 * (2 * kI8MaxStages + 6) + size_t(kI8TileN - p.rows) * kI8BlockK;
   p.stages = kI8MaxStages;
-  while (p.stages * stage + control > kI8MaxSmem) --p.stages;
+  while (p.stages > 1 && p.stages * stage + control > kI8MaxSmem) --p.stages;
   const size_t smem = p.stages * stage + control;
-  p.timeout_ns = g_timeout_ns;
   CUtensorMap map_w, map_q;
-  if (int rc = codes_map(&map_w, weight_codes, p.K, p.N, ldw, kI8TileN)) return rc;
+  if (int rc = codes_map(&map_w, weight_codes, p.K, p.N, ldw, static_cast<uint32_t>(p.rows))) return rc;
   if (int rc = codes_map(&map_q, codes, p.K, p.M, ldq, static_cast<uint32_t>(p.tok))) return rc;
   {
     std::lock_guard<std::mutex> lock(g_device_mutex);
     if (int rc = ensure_smem_attribute(configured[dev], int8_linear_kernel<kBf16>, kI8MaxSmem)) return rc;
   }
-  const int64_t tiles = tiles_m * tiles_n;
-  const int sms = usable_sms(info);
+  const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n;
   const int grid = static_cast<int>(tiles < sms ? tiles : sms);
   int8_linear_kernel<kBf16><<<grid, kI8Threads, smem, stream>>>(map_w, map_q, p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "8-bit linear launch");
   return FMM_OK;
+}
+
+template <bool kBf16>
+int launch_int8_pair(const int8_t* codes, int64_t ldq, const int8_t* weight_codes, int64_t ldw, Int8LinearParams p,
+                     int sms, cudaStream_t stream) {
+  using Cfg = Int8PairConfig;
+  static bool configured[kMaxDevices] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  p.tiles_m = static_cast<int32_t>(ceil_div(p.M, Cfg::kTile));
+  p.tiles_n = static_cast<int32_t>(ceil_div(p.N, Cfg::kTile));
+  CUtensorMap map_w, map_q, map_q16;
+  if (int rc = codes_map(&map_w, weight_codes, p.K, p.N, ldw, 128)) return rc;
+  if (int rc = codes_map(&map_q, codes, p.K, p.M, ldq, 128)) return rc;
+  if (int rc = codes_map(&map_q16, codes, p.K, p.M, ldq, 16)) return rc;
+  {
+    std::lock_guard<std::mutex> lock(g_device_mutex);
+    if (int rc = ensure_smem_attribute(configured[dev], int8_linear_pair_kernel<kBf16>, Cfg::kSmemBytes)) return rc;
+  }
+  const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n;
+  const int64_t pairs = tiles < sms / 2 ? tiles : sms / 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs), 1, 1);
+  cfg.blockDim = dim3(kI8Threads, 1, 1);
+  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, int8_linear_pair_kernel<kBf16>, map_w, map_q, map_q16, p);
+  if (e != cudaSuccess) return cuda_fail(e, "8-bit linear (pair) launch");
+  return FMM_OK;
+}
+
+constexpr size_t kI8FewShared = 216 * 1024;
+
+bool int8_few_fits(int64_t M, int64_t K) { return M * round_up(K, 16) <= int64_t(kI8FewShared / 2); }
+
+// Warps and stages of the few-token kernel beside the tokens' codes.
+void plan_int8_few(int64_t M, int64_t K, int64_t N, int channels, int sms, int* warps, int* stages, size_t* shared) {
+  const size_t tokens = static_cast<size_t>(M * round_up(K, 16));
+  // units of an SM, and as many warps as take an equal number of them
+  const int64_t each = ceil_div(ceil_div(N, channels), sms);
+  *warps = static_cast<int>(ceil_div(each, ceil_div(each, kI8FewMaxWarps)));
+  const size_t stage = size_t(channels) * kI8FewK, room = (kI8FewShared - tokens) / stage;
+  *stages = static_cast<int>(room / *warps);
+  if (*stages > kI8FewMaxStages) *stages = kI8FewMaxStages;
+  if (*stages < 2) {
+    *warps = static_cast<int>(room / 2);
+    *stages = 2;
+  }
+  *shared = *warps * *stages * stage + tokens;
+}
+
+template <bool kBf16, int MT, int R>
+int launch_int8_few(Int8FewParams p, int sms, cudaStream_t stream) {
+  static bool configured[kMaxDevices] = {};
+  auto kernel = int8_linear_few_kernel<kBf16, MT, R>;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  {
+    std::lock_guard<std::mutex> lock(g_device_mutex);
+    if (int rc = ensure_smem_attribute(configured[dev], kernel, kI8FewShared)) return rc;
+  }
+  int warps = 0;
+  size_t shared = 0;
+  plan_int8_few(p.M, p.K, p.N, R, sms, &warps, &p.stages, &shared);
+  const int64_t units = ceil_div(p.N, R);
+  p.units = static_cast<int32_t>(units);
+  const int grid = static_cast<int>(units < sms ? units : sms);
+  kernel<<<grid, 32 * warps, shared, stream>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "8-bit linear (few tokens) launch");
+  return FMM_OK;
+}
+
+// Channels of a unit of the few-token kernel: the most (4, 2, 1) that leave an
+// SM 12 units, so that enough warps have rows in flight.  One token, us for 1,
+// 2, 4: N = 12288, K = 4608: 19.5, 13.9, 12.8; N = 4096, K = 4096: 8.4, 6.8,
+// 7.1; N = 512, K = 4096: 4.3, 4.9, 6.2.
+int int8_few_channels(int64_t N, int sms) {
+  return N >= int64_t(48) * sms ? 4 : N >= int64_t(24) * sms ? 2 : 1;
+}
+
+template <bool kBf16, int MT>
+int launch_int8_few_tokens(const Int8FewParams& p, int channels, int sms, cudaStream_t stream) {
+  if (channels == 1) return launch_int8_few<kBf16, MT, 1>(p, sms, stream);
+  if (MT == 4 || channels == 2) return launch_int8_few<kBf16, MT, 2>(p, sms, stream);
+  if constexpr (MT < 4) return launch_int8_few<kBf16, MT, 4>(p, sms, stream);
+  return FMM_OK;
+}
+
+// Dot products for one or two tokens, and for three and four where the unit
+// has fewer than four channels (N = 4096, K = 4096, four tokens: 8.8 us, 9.6 on
+// the tensor cores; N = 12288, K = 4608: 16.7, 14.2); beyond that tensor cores,
+// by the estimates above.
+template <bool kBf16>
+int launch_linear_int8(const int8_t* codes, int64_t ldq, const int8_t* weight_codes, int64_t ldw,
+                       Int8LinearParams p, cudaStream_t stream) {
+  DeviceInfo* info = nullptr;
+  if (int rc = device_info(&info)) return rc;
+  const int sms = usable_sms(info);
+  p.group_m = 16;
+  p.timeout_ns = g_timeout_ns;
+  if (ceil_div(p.M, 16) * ceil_div(p.N, kI8TileN / 2) > (int64_t(1) << 30))
+    return fail(FMM_ERR_TOO_LARGE, "too many tiles");
+  const int channels = int8_few_channels(p.N, sms);
+  if ((p.M <= 2 || (p.M <= 4 && channels < 4)) && int8_few_fits(p.M, p.K)) {
+    Int8FewParams f = {};
+    f.codes = codes;
+    f.weight = weight_codes;
+    f.ldq = ldq;
+    f.ldw = ldw;
+    f.ldc = p.ldc;
+    f.N = p.N;
+    f.token_scales = p.token_scales;
+    f.channel_scales = p.channel_scales;
+    f.bias = p.bias;
+    f.out = p.out;
+    f.M = static_cast<int32_t>(p.M);
+    f.K = static_cast<int32_t>(p.K);
+    f.timeout_ns = g_timeout_ns;
+    if (p.M == 1) return launch_int8_few_tokens<kBf16, 1>(f, channels, sms, stream);
+    if (p.M == 2) return launch_int8_few_tokens<kBf16, 2>(f, channels, sms, stream);
+    return launch_int8_few_tokens<kBf16, 4>(f, channels, sms, stream);
+  }
+  double cost = 0;
+  const Int8Shape shape = choose_int8_shape(p.M, p.K, p.N, sms, &cost);
+  if (int8_pair_cost(p.M, p.K, p.N, sms) < cost)
+    return launch_int8_pair<kBf16>(codes, ldq, weight_codes, ldw, p, sms, stream);
+  return launch_int8_single<kBf16>(codes, ldq, weight_codes, ldw, p, shape, sms, stream);
 }
 
 // Device address of g_noalloc_scratch on the current device.  In host code the

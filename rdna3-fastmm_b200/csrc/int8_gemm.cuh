@@ -9,24 +9,22 @@
 // writes 32 consecutive outputs of one token, whatever N, ldc or the alignment
 // of Y (no vector store to fall back from).
 //
-// One CTA, persistent over the tiles:
-//   warp 0      TMA producer: a 128 x 128 box of W and a tok x 128 box of Q a
-//               stage (128-byte swizzle; what lies outside reads as zero).
-//   warp 1      MMA issuer: 4 x m128 n<tok> k32 a stage; owns TMEM.
-//   warps 2..5  epilogue: tcgen05.ld 32 lanes x 32 columns, scale, bias, one
-//               rounding, 64-byte row segments.
-// Every wait is bounded (mbar_wait_bounded).
+// Three kernels:
+//   int8_linear_few_kernel   a few tokens: bound by reading the weight
+//   int8_linear_kernel       one SM a tile of 8..128 channels x 16..256 tokens
+//   int8_linear_pair_kernel  two SMs a tile of 256 x 256 (many tokens)
+// Every wait is bounded (mbar_wait_bounded); on a timeout all roles unwind.
 #pragma once
 
 #include "fmm_common.cuh"
+#include "int8_rows.cuh"
 
 namespace fmm {
 
-constexpr int kI8TileN = 128;    // output channels of a tile
-constexpr int kI8BlockK = 128;   // k of a stage: one 128-byte swizzle row
+constexpr int kI8TileN = 128;    // output channels of an SM's tile
+constexpr int kI8BlockK = 128;   // k of one 128-byte swizzle row
 constexpr int kI8Threads = 192;
-constexpr uint32_t kI8WBytes = kI8TileN * kI8BlockK;
-constexpr int kI8MaxStages = 8;
+constexpr int kI8MaxStages = 24;
 
 struct Int8LinearParams {
   int64_t M, N, K;
@@ -37,10 +35,33 @@ struct Int8LinearParams {
   void* out;
   int32_t tok;       // tokens of a tile, a multiple of 16, <= 256
   int32_t stages;
+  int32_t rows;      // channels of a tile, a multiple of 8, <= 128
   int32_t tiles_m, tiles_n;
-  uint32_t tmem_cols;
+  int32_t group_m;   // token tiles of a group, which sweeps the channel tiles together
+  int32_t atoms;     // 128-deep columns of a stage
+  uint32_t tmem_cols;  // columns of one of the two accumulators
   uint64_t timeout_ns;
 };
+
+// True in one lane of a converged warp.  The loops around it are run by the
+// whole warp: with a single lane in them the compiler moves every descriptor
+// into uniform registers by loops of its own (4096-deep tiles of 64 channels x
+// 16 tokens: 13.7 us, 11.8 this way).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
+// Tile t -> (token tile, channel tile): groups of `group_m` token tiles sweep
+// the channel tiles, so that tiles in flight share tokens and weights in L2.
+__device__ __forceinline__ void int8_tile_coords(const Int8LinearParams& p, int t, int& tm, int& tn) {
+  const int per_group = p.group_m * p.tiles_n;
+  const int group = t / per_group, in_group = t - group * per_group;
+  const int first = group * p.group_m, rows = min(p.tiles_m - first, p.group_m);
+  tn = in_group / rows;
+  tm = first + in_group - tn * rows;
+}
 
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* tmap, uint32_t bar, int32_t c0,
                                             int32_t c1) {
@@ -58,6 +79,24 @@ __device__ __forceinline__ void tc_mma_i8(uint32_t d_tmem, uint64_t a_desc, uint
       "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 2-SM form, issued by one thread of the even CTA.
+__device__ __forceinline__ void tc_mma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap, uint32_t bar_cluster, int32_t c0,
+                                                 int32_t c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar_cluster), "r"(c0), "r"(c1)
       : "memory");
 }
 
@@ -80,6 +119,48 @@ __device__ __forceinline__ float load_bias(const void* bias, int64_t n) {
   return __half2float(static_cast<const __half*>(bias)[n]);
 }
 
+// Scaled outputs of 32 token columns for one lane's channel: column c + j of
+// the tile is token m0 + c + j, lane j holds its scale.  A tile's columns are converted by one warp
+// each, so instructions count: whole blocks of 32 tokens x 32 channels take two
+// columns to a conversion and no predicates (9 instructions a column; 25 with a
+// branch a store, which held the 256 x 256 tiles back: 4096 x 4096 x 12288
+// 176 us).
+template <bool kBf16>
+__device__ __forceinline__ void store_columns(const Int8LinearParams& p, const uint32_t (&v)[32], int64_t m0, int c,
+                                              int tokens, int64_t n, float token_scale, float channel_scale, float bias) {
+  uint16_t* out = static_cast<uint16_t*>(p.out) + (m0 + c) * p.ldc + n;
+  const int64_t ldc = p.ldc;
+  if (c + 32 <= tokens && __all_sync(0xffffffffu, n < p.N)) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+      const float a = __shfl_sync(0xffffffffu, token_scale, j), b = __shfl_sync(0xffffffffu, token_scale, j + 1);
+      const uint32_t two =
+          pack2_rn<kBf16>(fmaf(static_cast<float>(static_cast<int32_t>(v[j])), a * channel_scale, bias),
+                          fmaf(static_cast<float>(static_cast<int32_t>(v[j + 1])), b * channel_scale, bias));
+      out[0] = static_cast<uint16_t>(two);
+      out[ldc] = static_cast<uint16_t>(two >> 16);
+      out += 2 * ldc;
+    }
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    const float ts = __shfl_sync(0xffffffffu, token_scale, j);
+    if (c + j < tokens && n < p.N) out[j * ldc] = int8_output<kBf16>(v[j], ts, channel_scale, bias);
+  }
+}
+
+// Structure (persistent over the tiles; 2 x tmem_cols accumulator columns, so
+// that the epilogue of a tile runs beside the next one's products):
+//   warp 0      TMA producer: a rows x 128 box of W and a tok x 128 box of Q a
+//               stage (128-byte swizzle; what lies outside reads as zero).
+//   warp 1      MMA issuer: 4 x m128 n<tok> k32 a stage; owns TMEM.
+//   warps 2..5  epilogue: tcgen05.ld 32 lanes x 32 columns, scale, bias, one
+//               rounding, 64-byte row segments.
+// A tile may have fewer than 128 channels, so that a few tokens' tiles, which
+// cost the weight's bytes and little else, come out even over the SMs; the
+// product runs over 128 rows of shared memory all the same and the sums of the
+// rows behind the tile, whatever they are, are not read.
 template <bool kBf16>
 __global__ void __launch_bounds__(kI8Threads, 1)
     int8_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_q,
@@ -88,34 +169,80 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
   const uint32_t tok_bytes = static_cast<uint32_t>(p.tok) * kI8BlockK;
-  const uint32_t stage_bytes = kI8WBytes + tok_bytes;
-  uint8_t* ctrl = smem_raw + (base - raw_addr) + p.stages * stage_bytes;
+  const uint32_t w_bytes = static_cast<uint32_t>(p.rows) * kI8BlockK;
+  const uint32_t stage_bytes = p.atoms * (w_bytes + tok_bytes);
+  // tokens first: the products read 128 rows of W, into the next stage or, at
+  // the end, into what the host adds behind the last one
+  uint8_t* ctrl = smem_raw + (base - raw_addr) + p.stages * stage_bytes + (kI8TileN - p.rows) * kI8BlockK;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ctrl);
   const uint32_t full_bar = smem_u32(bars);
   const uint32_t empty_bar = smem_u32(bars + kI8MaxStages);
-  const uint32_t tfull_bar = smem_u32(bars + 2 * kI8MaxStages);
-  const uint32_t tempty_bar = smem_u32(bars + 2 * kI8MaxStages + 1);
-  const uint32_t drain_bar = smem_u32(bars + 2 * kI8MaxStages + 2);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kI8MaxStages + 3);
+  const uint32_t tfull_bar = smem_u32(bars + 2 * kI8MaxStages);       // [2]
+  const uint32_t tempty_bar = smem_u32(bars + 2 * kI8MaxStages + 2);  // [2]
+  const uint32_t drain_bar = smem_u32(bars + 2 * kI8MaxStages + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kI8MaxStages + 5);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
+  const int total = p.tiles_m * p.tiles_n;
+  const int columns = static_cast<int>((p.K + kI8BlockK - 1) / kI8BlockK);  // 128 codes each
+
+  // the producer's place: tile, column, stage; one call waits for a stage, loads it and moves on
+  int load_t = blockIdx.x, load_kb = 0, load_stage = 0, issued = 0, load_m = 0, load_n = 0;
+  uint32_t load_phase = 0;
+  bool load_ok = true;
+  if (load_t < total) int8_tile_coords(p, load_t, load_m, load_n);
+  auto load_stage_next = [&] {
+    load_ok = __all_sync(0xffffffffu, mbar_wait_bounded(empty_bar + 8 * load_stage, load_phase ^ 1u, abort,
+                                                        p.timeout_ns, 21));
+    if (!load_ok) return;
+    if (elect_one()) {
+      const int atoms = min(p.atoms, columns - load_kb);
+      const uint32_t bar = full_bar + 8 * load_stage;
+      uint32_t dst = base + load_stage * stage_bytes;
+      mbar_arrive_expect_tx(bar, atoms * (w_bytes + tok_bytes));
+      for (int at = 0; at < atoms; ++at) {
+        tma_load_2d(dst + tok_bytes, &tmap_w, bar, (load_kb + at) * kI8BlockK, load_n * p.rows);
+        tma_load_2d(dst, &tmap_q, bar, (load_kb + at) * kI8BlockK, load_m * p.tok);
+        dst += w_bytes + tok_bytes;
+      }
+    }
+    __syncwarp();
+    ++issued;
+    if (++load_stage == p.stages) {
+      load_stage = 0;
+      load_phase ^= 1u;
+    }
+    if ((load_kb += p.atoms) >= columns) {
+      load_kb = 0;
+      load_t += gridDim.x;
+      if (load_t < total) int8_tile_coords(p, load_t, load_m, load_n);
+    }
+  };
+
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(full_bar + 8 * s, 1);
       mbar_init(empty_bar + 8 * s, 1);
     }
-    mbar_init(tfull_bar, 1);
-    mbar_init(tempty_bar, 4);  // one arrival per epilogue warp
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(tfull_bar + 8 * b, 1);
+      mbar_init(tempty_bar + 8 * b, 4);  // one arrival per epilogue warp
+    }
     mbar_init(drain_bar, 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     prefetch_tmap(&tmap_w);
     prefetch_tmap(&tmap_q);
   }
+  if (warp == 0) {
+    // the ring is filled while tensor memory is being allocated
+    __syncwarp();
+    while (issued < p.stages && load_t < total && load_ok) load_stage_next();
+  }
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), p.tmem_cols);
+    tmem_alloc(smem_u32(tmem_slot), 2 * p.tmem_cols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -123,120 +250,109 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  const int total = p.tiles_m * p.tiles_n;
-  const int k_blocks = static_cast<int>((p.K + kI8BlockK - 1) / kI8BlockK);
-
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0, issued = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-        const int tm = t / p.tiles_n, tn = t - tm * p.tiles_n;
-        for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!mbar_wait_bounded(empty_bar + 8 * stage, phase ^ 1u, abort, p.timeout_ns, 21)) {
-            ok = false;
-            break;
-          }
-          const uint32_t dst = base + stage * stage_bytes;
-          mbar_arrive_expect_tx(full_bar + 8 * stage, stage_bytes);
-          tma_load_2d(dst, &tmap_w, full_bar + 8 * stage, kb * kI8BlockK, tn * kI8TileN);
-          tma_load_2d(dst + kI8WBytes, &tmap_q, full_bar + 8 * stage, kb * kI8BlockK, tm * p.tok);
-          ++issued;
-          if (++stage == p.stages) {
-            stage = 0;
-            phase ^= 1u;
-          }
+    while (load_t < total && load_ok) load_stage_next();
+    if (!load_ok) {
+      // the last min(stages, issued) loads may still be landing
+      for (int n = 0; n < p.stages && n < issued; ++n) {
+        if (--load_stage < 0) {
+          load_stage = p.stages - 1;
+          load_phase ^= 1u;
         }
-      }
-      if (!ok) {
-        // the last min(stages, issued) loads may still be landing
-        int s = stage;
-        uint32_t ph = phase;
-        for (int n = 0; n < p.stages && n < issued; ++n) {
-          if (--s < 0) {
-            s = p.stages - 1;
-            ph ^= 1u;
-          }
-          volatile int no_abort = 0;
-          mbar_wait_bounded(full_bar + 8 * s, ph, &no_abort, p.timeout_ns, 25);
-        }
+        volatile int no_abort = 0;
+        mbar_wait_bounded(full_bar + 8 * load_stage, load_phase, &no_abort, p.timeout_ns, 25);
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0, acc_phase = 0;
-      bool ok = true, issued_any = false;
-      const uint32_t idesc = idesc_i8_s32(kI8TileN, static_cast<uint32_t>(p.tok));
-      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
-        if (!mbar_wait_bounded(tempty_bar, acc_phase ^ 1u, abort, p.timeout_ns, 22)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        for (int kb = 0; kb < k_blocks; ++kb) {
-          if (!mbar_wait_bounded(full_bar + 8 * stage, phase, abort, p.timeout_ns, 23)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint32_t src = base + stage * stage_bytes;
-#pragma unroll
-          for (int kk = 0; kk < kI8BlockK / 32; ++kk)
-            tc_mma_i8(tmem_base, smem_desc_k_sw128(src + kk * 32), smem_desc_k_sw128(src + kI8WBytes + kk * 32),
-                      idesc, (kb > 0 || kk > 0) ? 1u : 0u);
-          issued_any = true;
-          tc_commit(empty_bar + 8 * stage);
-          if (++stage == p.stages) {
-            stage = 0;
-            phase ^= 1u;
-          }
-        }
+    int stage = 0, acc = 0;
+    uint32_t phase = 0, acc_phase = 0;
+    bool ok = true, issued_any = false;
+    const uint32_t idesc = idesc_i8_s32(kI8TileN, static_cast<uint32_t>(p.tok));
+    const uint64_t q_desc0 = smem_desc_k_sw128(base), w_desc0 = smem_desc_k_sw128(base + tok_bytes);
+    const uint32_t atom_step = (w_bytes + tok_bytes) >> 4, stage_step = stage_bytes >> 4;
+    for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      ok = __all_sync(0xffffffffu, mbar_wait_bounded(tempty_bar + 8 * acc, acc_phase ^ 1u, abort, p.timeout_ns, 22));
+      if (!ok) break;
+      tc_fence_after();
+      const uint32_t d_tmem = tmem_base + acc * p.tmem_cols;
+      for (int kb = 0; kb < columns; kb += p.atoms) {
+        ok = __all_sync(0xffffffffu, mbar_wait_bounded(full_bar + 8 * stage, phase, abort, p.timeout_ns, 23));
         if (!ok) break;
-        tc_commit(tfull_bar);
+        tc_fence_after();
+        if (elect_one()) {
+          const int atoms = min(p.atoms, columns - kb);
+          uint64_t q_desc = q_desc0 + stage * stage_step, w_desc = w_desc0 + stage * stage_step;
+          for (int at = 0; at < atoms; ++at) {
+#pragma unroll
+            for (int kk = 0; kk < kI8BlockK / 32; ++kk)  // 32 codes on, 32 bytes on
+              tc_mma_i8(d_tmem, w_desc + kk * 2, q_desc + kk * 2, idesc, (kb > 0 || at > 0 || kk > 0) ? 1u : 0u);
+            q_desc += atom_step;
+            w_desc += atom_step;
+          }
+          tc_commit(empty_bar + 8 * stage);
+        }
+        __syncwarp();
+        issued_any = true;
+        if (++stage == p.stages) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+      if (!ok) break;
+      if (elect_one()) tc_commit(tfull_bar + 8 * acc);
+      __syncwarp();
+      if (++acc == 2) {
+        acc = 0;
         acc_phase ^= 1u;
       }
-      if (!ok && issued_any) {
-        tc_commit(drain_bar);
-        volatile int no_abort = 0;
-        mbar_wait_bounded(drain_bar, 0, &no_abort, p.timeout_ns, 26);
-      }
+    }
+    if (!ok && issued_any) {
+      if (elect_one()) tc_commit(drain_bar);
+      __syncwarp();
+      volatile int no_abort = 0;
+      mbar_wait_bounded(drain_bar, 0, &no_abort, p.timeout_ns, 26);
     }
   } else {
     const int quarter = warp & 3;  // TMEM lanes this warp may access
+    int acc = 0;
     uint32_t acc_phase = 0;
-    uint16_t* out = static_cast<uint16_t*>(p.out);
     for (int t = blockIdx.x; t < total; t += gridDim.x) {
-      const int tm = t / p.tiles_n, tn = t - tm * p.tiles_n;
-      const int64_t n = static_cast<int64_t>(tn) * kI8TileN + quarter * 32 + lane;
+      int tm, tn;
+      int8_tile_coords(p, t, tm, tn);
+      const int row = quarter * 32 + lane;
+      // a lane behind the tile has no channel
+      const int64_t n = row < p.rows ? static_cast<int64_t>(tn) * p.rows + row : p.N;
       const int64_t m0 = static_cast<int64_t>(tm) * p.tok;
       const int tokens = static_cast<int>(p.M - m0 < p.tok ? p.M - m0 : p.tok);
       const float channel_scale = n < p.N ? p.channel_scales[n] : 0.0f;
       const float bias = n < p.N ? load_bias<kBf16>(p.bias, n) : 0.0f;
+      float token_scale = lane < tokens ? p.token_scales[m0 + lane] : 0.0f;
       int ready = 0;
-      if (lane == 0) ready = mbar_wait_bounded(tfull_bar, acc_phase, abort, p.timeout_ns, 24) ? 1 : 0;
+      if (lane == 0) ready = mbar_wait_bounded(tfull_bar + 8 * acc, acc_phase, abort, p.timeout_ns, 24) ? 1 : 0;
       ready = __shfl_sync(0xffffffffu, ready, 0);
       if (!ready) break;
       tc_fence_after();
-      const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+      const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * p.tmem_cols;
+      if (quarter * 32 < p.rows) {
 #pragma unroll 1
-      for (int c = 0; c < tokens; c += 32) {
-        uint32_t v[32];
-        tc_ld_32x32b_x32(t_addr + c, v);
-        tc_wait_ld();
-        const float token_scale = c + lane < tokens ? p.token_scales[m0 + c + lane] : 0.0f;
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const float ts = __shfl_sync(0xffffffffu, token_scale, j);
-          if (c + j < tokens && n < p.N)
-            out[(m0 + c + j) * p.ldc + n] = int8_output<kBf16>(v[j], ts, channel_scale, bias);
+        for (int c = 0; c < tokens; c += 32) {
+          uint32_t v[32];
+          tc_ld_32x32b_x32(t_addr + c, v);
+          // the next columns' scales, before they are waited for
+          const int next = c + 32 + lane;
+          const float next_scale = next < tokens ? p.token_scales[m0 + next] : 0.0f;
+          tc_wait_ld();
+          store_columns<kBf16>(p, v, m0, c, tokens, n, token_scale, channel_scale, bias);
+          token_scale = next_scale;
         }
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(tempty_bar);
-      acc_phase ^= 1u;
+      if (lane == 0) mbar_arrive(tempty_bar + 8 * acc);
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
     }
   }
 
@@ -244,7 +360,393 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, p.tmem_cols);
+    tmem_dealloc(tmem_base, 2 * p.tmem_cols);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// 2-SM form: a cluster of two CTAs computes a tile of 256 channels x 256 tokens
+// with tcgen05.mma.cta_group::2.  CTA r holds channels [128 r, 128 r + 128) of
+// the W tile and its half of the tokens, so an SM loads 32 KB a 128-deep block
+// for twice the products that the same bytes give one SM alone: at the full
+// rate L2 and shared memory are what bounds the product, not the tensor cores.
+// Roles as above; the even CTA issues the products, loads complete on its
+// barriers, and each CTA's epilogue drains its own 128 channels.
+struct Int8PairConfig {
+  static constexpr int kTile = 256;
+  static constexpr int kAtoms = 2;  // 128-deep columns of swizzle atoms a stage
+  static constexpr int kBK = kAtoms * kI8BlockK;
+  static constexpr int kStages = 3;
+  static constexpr uint32_t kAtomBytes = 128 * kI8BlockK;      // this CTA's half of W or Q
+  static constexpr uint32_t kABytes = kAtoms * kAtomBytes;     // 32 KB
+  static constexpr uint32_t kStageBytes = 2 * kABytes;         // 64 KB
+  static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + 1024 + 8 * (2 * kStages + 8);
+};
+
+template <bool kBf16>
+__global__ void __launch_bounds__(kI8Threads, 1)
+    int8_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_q,
+                            const __grid_constant__ CUtensorMap tmap_q16, const Int8LinearParams p) {
+  using Cfg = Int8PairConfig;
+  constexpr int STAGES = Cfg::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_u32(smem_raw);
+  const uint32_t base = (raw_addr + 1023u) & ~1023u;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + (base - raw_addr) + STAGES * Cfg::kStageBytes);
+  const uint32_t full_bar = smem_u32(bars);                     // [STAGES], used in CTA 0
+  const uint32_t empty_bar = smem_u32(bars + STAGES);           // [STAGES], each CTA
+  const uint32_t tfull_bar = smem_u32(bars + 2 * STAGES);       // [2], each CTA
+  const uint32_t tempty_bar = smem_u32(bars + 2 * STAGES + 2);  // [2], used in CTA 0
+  const uint32_t drain_bar = smem_u32(bars + 2 * STAGES + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 5);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32;
+  const int lane = threadIdx.x % 32;
+  const uint32_t cta = cluster_cta_rank();  // 0 = even CTA (issues the MMAs)
+  const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar + 8 * s, 1);
+      mbar_init(empty_bar + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(tfull_bar + 8 * b, 1);
+      mbar_init(tempty_bar + 8 * b, 8);  // 4 epilogue warps x 2 CTAs
+    }
+    mbar_init(drain_bar, 1);
+    *abort = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    prefetch_tmap(&tmap_w);
+    prefetch_tmap(&tmap_q);
+    prefetch_tmap(&tmap_q16);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), 2 * Cfg::kTile);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync_all();  // barriers of both CTAs initialised, TMEM allocated
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int total = p.tiles_m * p.tiles_n;
+  const int k_blocks = static_cast<int>((p.K + Cfg::kBK - 1) / Cfg::kBK);
+  // token columns of tile tm: the MMA's N, 16 from each CTA at least
+  auto columns = [&](int tm) {
+    const int64_t rest = p.M - static_cast<int64_t>(tm) * Cfg::kTile;
+    return rest >= Cfg::kTile ? Cfg::kTile : static_cast<int>((rest + 31) / 32 * 32);
+  };
+
+  if (warp == 0) {
+    int stage = 0, issued = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int t = pair; t < total && ok; t += pairs) {
+      int tm, tn;
+      int8_tile_coords(p, t, tm, tn);
+      // each CTA supplies half of the tokens; a ragged last tile loads
+      // exactly its half in 16-row boxes, since a 128-row box would fetch
+      // rows that belong to the other half
+      const int n_cols = columns(tm), half = n_cols / 2;
+      const int w_row = tn * Cfg::kTile + static_cast<int>(cta) * 128;
+      const int q_row = tm * Cfg::kTile + static_cast<int>(cta) * half;
+      const uint32_t stage_tx = 2u * (Cfg::kABytes + static_cast<uint32_t>(half) * Cfg::kBK);
+      for (int kb = 0; kb < k_blocks; ++kb) {
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait_bounded_cluster(empty_bar + 8 * stage, phase ^ 1u, abort, p.timeout_ns, 41));
+        if (!ok) break;
+        if (elect_one()) {
+          const uint32_t full_even = map_to_cta(full_bar + 8 * stage, 0);
+          if (cta == 0) mbar_arrive_expect_tx(full_bar + 8 * stage, stage_tx);
+#pragma unroll
+          for (int at = 0; at < Cfg::kAtoms; ++at) {
+            const int k0 = kb * Cfg::kBK + at * kI8BlockK;
+            const uint32_t w_dst = base + stage * Cfg::kStageBytes + at * Cfg::kAtomBytes;
+            const uint32_t q_dst = w_dst + Cfg::kABytes;
+            tma_load_2d_pair(w_dst, &tmap_w, full_even, k0, w_row);
+            if (n_cols == Cfg::kTile) {
+              tma_load_2d_pair(q_dst, &tmap_q, full_even, k0, q_row);
+            } else {
+              for (int j = 0; j < half; j += 16)
+                tma_load_2d_pair(q_dst + static_cast<uint32_t>(j) * kI8BlockK, &tmap_q16, full_even, k0, q_row + j);
+            }
+          }
+        }
+        __syncwarp();
+        ++issued;
+        if (++stage == STAGES) {
+          stage = 0;
+          phase ^= 1u;
+        }
+      }
+    }
+    if (!ok && issued > 0) {
+      // loads may still be landing in this CTA's shared memory (they complete
+      // on the even CTA's barrier): give them time before the CTA unwinds
+      const uint64_t start = globaltimer_ns();
+      while (globaltimer_ns() - start < 200000ull) {
+      }
+    }
+  } else if (warp == 1) {
+    if (cta == 0) {
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true, issued_any = false;
+      const uint64_t w_desc0 = smem_desc_k_sw128(base), q_desc0 = smem_desc_k_sw128(base + Cfg::kABytes);
+      for (int t = pair; t < total && ok; t += pairs) {
+        int tm, tn;
+        int8_tile_coords(p, t, tm, tn);
+        const uint32_t idesc = idesc_i8_s32(Cfg::kTile, static_cast<uint32_t>(columns(tm)));
+        ok = __all_sync(0xffffffffu,
+                        mbar_wait_bounded_cluster(tempty_bar + 8 * acc, acc_phase ^ 1u, abort, p.timeout_ns, 42));
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + static_cast<uint32_t>(acc * Cfg::kTile);
+        for (int kb = 0; kb < k_blocks; ++kb) {
+          ok = __all_sync(0xffffffffu,
+                          mbar_wait_bounded_cluster(full_bar + 8 * stage, phase, abort, p.timeout_ns, 43));
+          if (!ok) break;
+          tc_fence_after();
+          if (elect_one()) {
+            const uint64_t w_desc = w_desc0 + stage * (Cfg::kStageBytes >> 4);
+            const uint64_t q_desc = q_desc0 + stage * (Cfg::kStageBytes >> 4);
+#pragma unroll
+            for (int kk = 0; kk < Cfg::kBK / 32; ++kk) {
+              const uint32_t at = (kk / 4) * (Cfg::kAtomBytes >> 4) + (kk % 4) * 2;
+              tc_mma_i8_pair(d_tmem, w_desc + at, q_desc + at, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+            }
+            tc_commit_pair_multicast(empty_bar + 8 * stage, 0x3);
+          }
+          __syncwarp();
+          issued_any = true;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1u;
+          }
+        }
+        if (!ok) break;
+        if (elect_one()) tc_commit_pair_multicast(tfull_bar + 8 * acc, 0x3);
+        __syncwarp();
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1u;
+        }
+      }
+      if (!ok && issued_any) {
+        if (elect_one()) tc_commit_pair_multicast(drain_bar, 0x1);
+        __syncwarp();
+        volatile int no_abort = 0;
+        mbar_wait_bounded(drain_bar, 0, &no_abort, p.timeout_ns, 46);
+      }
+    }
+  } else {
+    const int quarter = warp & 3;
+    const uint32_t tempty_even = map_to_cta(tempty_bar, 0);
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    for (int t = pair; t < total; t += pairs) {
+      int tm, tn;
+      int8_tile_coords(p, t, tm, tn);
+      const int64_t n = static_cast<int64_t>(tn) * Cfg::kTile + static_cast<int>(cta) * 128 + quarter * 32 + lane;
+      const int64_t m0 = static_cast<int64_t>(tm) * Cfg::kTile;
+      const int tokens = static_cast<int>(p.M - m0 < Cfg::kTile ? p.M - m0 : Cfg::kTile);
+      const float channel_scale = n < p.N ? p.channel_scales[n] : 0.0f;
+      const float bias = n < p.N ? load_bias<kBf16>(p.bias, n) : 0.0f;
+      float token_scale = lane < tokens ? p.token_scales[m0 + lane] : 0.0f;
+      int ready = 0;
+      if (lane == 0)
+        ready = mbar_wait_bounded_cluster(tfull_bar + 8 * acc, acc_phase, abort, p.timeout_ns, 44) ? 1 : 0;
+      ready = __shfl_sync(0xffffffffu, ready, 0);
+      if (!ready) break;
+      tc_fence_after();
+      const uint32_t t_addr =
+          tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * Cfg::kTile);
+#pragma unroll 1
+      for (int c = 0; c < tokens; c += 32) {
+        uint32_t v[32];
+        tc_ld_32x32b_x32(t_addr + c, v);
+        const int next = c + 32 + lane;
+        const float next_scale = next < tokens ? p.token_scales[m0 + next] : 0.0f;
+        tc_wait_ld();
+        store_columns<kBf16>(p, v, m0, c, tokens, n, token_scale, channel_scale, bias);
+        token_scale = next_scale;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_remote(tempty_even + 8 * acc);
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1u;
+      }
+    }
+  }
+
+  tc_fence_before();
+  cluster_sync_all();  // nobody leaves while the pair may still touch its memory
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_base, 2 * Cfg::kTile);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Few tokens: Y = Q W^T is bound by reading W once, and by the time from the
+// launch to the last store.  Nothing is shared between warps: each takes units
+// of four channels in turn, whose rows come through a ring of its own in shared
+// memory by bulk copies (issued by the warp itself, running on across units),
+// against the tokens' codes, which the CTA keeps in shared memory.  Products
+// are dot products of four codes; a lane sums every 32nd 16-code piece of a
+// row, and the lanes' 32-bit sums are added at the row's end.  Units of four
+// channels spread W over all SMs (tiles of 128 leave a third of them idle at
+// N = 12288), and neither tensor maps nor tensor memory are set up first.
+//   MT: tokens, rounded up.
+constexpr int kI8FewK = 1024;  // codes of a row in a stage
+constexpr int kI8FewMaxWarps = 16, kI8FewMaxStages = 8;
+
+struct Int8FewParams {
+  const int8_t* codes;
+  const int8_t* weight;
+  int64_t ldq, ldw, ldc, N;
+  const float* token_scales;
+  const float* channel_scales;
+  const void* bias;
+  void* out;
+  int32_t M, K;
+  int32_t units, stages;
+  uint64_t timeout_ns;
+};
+
+// 16 codes of a row from `k` on; what lies past K is zero and not read.
+__device__ __forceinline__ uint4 load_codes(const int8_t* row, int k, int K) {
+  if (k + 16 <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
+  uint32_t w[4] = {0, 0, 0, 0};
+  if (k < K) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (k + i < K) w[i / 4] |= static_cast<uint32_t>(static_cast<uint8_t>(row[k + i])) << (8 * (i % 4));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ int dot16(const uint4& a, const uint4& b, int c) {
+  c = __dp4a(static_cast<int>(a.x), static_cast<int>(b.x), c);
+  c = __dp4a(static_cast<int>(a.y), static_cast<int>(b.y), c);
+  c = __dp4a(static_cast<int>(a.z), static_cast<int>(b.z), c);
+  return __dp4a(static_cast<int>(a.w), static_cast<int>(b.w), c);
+}
+
+template <bool kBf16, int MT, int R>
+__global__ void __launch_bounds__(32 * kI8FewMaxWarps, 1) int8_linear_few_kernel(const Int8FewParams p) {
+  constexpr uint32_t kStageBytes = R * kI8FewK;
+  static_assert(MT * R <= 32, "an output a lane");
+  __shared__ __align__(8) uint64_t s_full[kI8FewMaxWarps * kI8FewMaxStages];
+  __shared__ int s_abort[kI8FewMaxWarps];
+  extern __shared__ __align__(128) uint8_t s_few[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+  const uint32_t full_bar = smem_u32(s_full + warp * kI8FewMaxStages);
+  const int pitch = (p.K + 15) / 16 * 16;  // of a token's codes
+  uint8_t* ring = s_few + warp * p.stages * kStageBytes;
+  uint8_t* tokens = s_few + warps * p.stages * kStageBytes;
+  const int k_stages = (p.K + kI8FewK - 1) / kI8FewK;
+  const int whole = p.K & ~15;  // codes that copies move; the rest of a row is read in place
+
+  // this warp's units and stages, in the order in which they are copied
+  const int unit0 = warp * gridDim.x + blockIdx.x, unit_step = warps * gridDim.x;
+  int copy_unit = unit0, copy_ks = 0;
+  auto copy = [&](int stage) {
+    if (copy_unit >= p.units) return;
+    const int64_t n0 = static_cast<int64_t>(copy_unit) * R;
+    const int rows = static_cast<int>(p.N - n0 < R ? p.N - n0 : R), k0 = copy_ks * kI8FewK;
+    const int bytes = max(0, min(kI8FewK, whole - k0));
+    const uint32_t bar = full_bar + 8 * stage;
+    if (lane == 0) mbar_arrive_expect_tx(bar, static_cast<uint32_t>(rows * bytes));
+    __syncwarp();
+    if (lane < rows && bytes > 0)
+      bulk_load(smem_u32(ring) + stage * kStageBytes + lane * kI8FewK, p.weight + (n0 + lane) * p.ldw + k0,
+                static_cast<uint32_t>(bytes), bar);
+    if (++copy_ks == k_stages) {
+      copy_ks = 0;
+      copy_unit += unit_step;
+    }
+  };
+  if (lane == 0) {
+    s_abort[warp] = 0;
+    for (int s = 0; s < p.stages; ++s) mbar_init(full_bar + 8 * s, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
+  for (int s = 0; s < p.stages; ++s) copy(s);
+  // the tokens, zero past K
+  for (int i = threadIdx.x; i < p.M * (pitch / 16); i += blockDim.x) {
+    const int m = i / (pitch / 16), k = (i - m * (pitch / 16)) * 16;
+    *reinterpret_cast<uint4*>(tokens + m * pitch + k) = load_codes(p.codes + m * p.ldq, k, p.K);
+  }
+  // lane m * R + r stores the output of token m and channel r of the unit
+  const int out_m = lane / R, out_r = lane % R;
+  const float token_scale = out_m < p.M ? p.token_scales[out_m] : 0.0f;
+  __syncthreads();
+
+  int stage = 0;
+  uint32_t phase = 0;
+  for (int unit = unit0; unit < p.units; unit += unit_step) {
+    const int64_t n0 = static_cast<int64_t>(unit) * R, n = n0 + out_r;
+    const float channel_scale = n < p.N ? p.channel_scales[n] : 0.0f;
+    const float bias = n < p.N ? load_bias<kBf16>(p.bias, n) : 0.0f;
+    int sum[MT][R];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < R; ++r) sum[m][r] = 0;
+    for (int ks = 0; ks < k_stages; ++ks) {
+      mbar_wait_bounded(full_bar + 8 * stage, phase, &s_abort[warp], p.timeout_ns, 51);
+      const uint8_t* from = ring + stage * kStageBytes;
+#pragma unroll
+      for (int i = 0; i < kI8FewK / 512; ++i) {
+        const int at = i * 512 + lane * 16, k = ks * kI8FewK + at;
+        if (k >= p.K) continue;
+        uint4 w[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) w[r] = *reinterpret_cast<const uint4*>(from + r * kI8FewK + at);
+        if (k >= whole) {
+#pragma unroll
+          for (int r = 0; r < R; ++r)
+            w[r] = n0 + r < p.N ? load_codes(p.weight + (n0 + r) * p.ldw, k, p.K) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          if (m >= p.M) break;
+          const uint4 q = *reinterpret_cast<const uint4*>(tokens + m * pitch + k);
+#pragma unroll
+          for (int r = 0; r < R; ++r) sum[m][r] = dot16(w[r], q, sum[m][r]);
+        }
+      }
+      // all lanes hold their pieces: the stage may be filled again
+      if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&s_abort[warp]) != 0)) break;
+      copy(stage);
+      if (++stage == p.stages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    if (__any_sync(0xffffffffu, *static_cast<volatile int*>(&s_abort[warp]) != 0)) break;
+    int mine = 0;
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int all = __reduce_add_sync(0xffffffffu, sum[m][r]);
+        mine = lane == m * R + r ? all : mine;
+      }
+    if (out_m < p.M && n < p.N)
+      static_cast<uint16_t*>(p.out)[out_m * p.ldc + n] =
+          int8_output<kBf16>(static_cast<uint32_t>(mine), token_scale, channel_scale, bias);
+  }
+  if (s_abort[warp] != 0 && lane == 0) {
+    // copies into this warp's ring may still be landing: give each its limit
+    volatile int no_abort = 0;
+    for (int s = 0; s < p.stages; ++s)
+      mbar_wait_bounded(full_bar + 8 * s, s < stage ? phase ^ 1u : phase, &no_abort, p.timeout_ns, 52);
   }
 }
 

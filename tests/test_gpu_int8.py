@@ -282,7 +282,12 @@ def _run_linear(codes, scales, w, ws, bias, dtype, **kw):
 SHAPES = [(1, 1, 1), (1, 128, 128), (2, 17, 31), (7, 129, 300), (15, 16, 129), (16, 4097, 127), (17, 300, 257),
           (31, 1000, 33), (33, 640, 1000), (64, 2048, 512), (80, 513, 640), (100, 96, 2000), (128, 4096, 256),
           (129, 384, 385), (255, 256, 130), (256, 128, 512), (257, 263, 269), (520, 776, 392), (1000, 200, 1),
-          (1025, 1152, 2049), (2050, 64, 300), (1, 16384, 4096), (3, 70000, 40)]
+          (1025, 1152, 2049), (2050, 64, 300), (1, 16384, 4096), (3, 70000, 40),
+          # each kernel, its widths and its ends: few tokens by 1, 2 and 4 channels, tiles of 64 and
+          # 128 channels, pairs of SMs with whole and ragged token tiles
+          (1, 1040, 500), (2, 2063, 4001), (4, 1025, 3600), (4, 4096, 131), (1, 4609, 8001), (2, 1024, 7300),
+          (5, 300, 9000), (48, 1100, 8200), (200, 2000, 4100), (700, 515, 9001), (600, 4096, 9472),
+          (1300, 1031, 4999), (300, 1024, 37889)]
 
 
 @pytest.mark.parametrize("with_bias", [False, True])
