@@ -259,34 +259,11 @@ def linear(scheme: str, A, W, bias, C, L, Rt, P, prepacked: bool, right_kn: bool
           "fmm_linear")
 
 
-def row_dtype_id(dtype) -> int:
-    """Element type of a row operand of the 8-bit operators."""
-    import torch
-
-    ids = {torch.bfloat16: FMM_DTYPE_BF16, torch.float16: FMM_DTYPE_F16, torch.float32: FMM_DTYPE_F32}
-    if dtype not in ids:
-        raise ValueError(f"the 8-bit operators take BF16, FP16 or (where they say so) FP32, not {dtype}")
-    return ids[dtype]
-
-
-def quantize_rows(dtype: int, x: int, rows: int, cols: int, ldx: int, codes: int, ldq: int, scales: int,
-                  stream: int) -> None:
-    """Addresses and leading dimensions, as the C ABI takes them: the 8-bit
-    operators run between single tokens, where a call's own time counts."""
-    check(library().fmm_quantize_rows(dtype, x, rows, cols, ldx, codes, ldq, scales, stream), "fmm_quantize_rows")
-
-
-def rms_norm_int8(dtype: int, gain_dtype: int, x: int, ldx: int, residual: int | None, ldr: int, gain: int,
-                  rows: int, cols: int, eps: float, residual_out: int | None, ldo: int, codes: int, ldq: int,
-                  scales: int, stream: int) -> None:
-    check(library().fmm_rms_norm_int8(dtype, gain_dtype, x, ldx, residual, ldr, gain, rows, cols, eps,
-                                      residual_out, ldo, codes, ldq, scales, stream), "fmm_rms_norm_int8")
-
-
-def linear_int8(dtype: int, codes: int, ldq: int, scales: int, weight_codes: int, ldw: int, weight_scales: int,
-                bias: int | None, out: int, ldc: int, rows: int, inner: int, columns: int, stream: int) -> None:
-    check(library().fmm_linear_int8(dtype, codes, ldq, scales, weight_codes, ldw, weight_scales, bias, out, ldc,
-                                    rows, inner, columns, stream), "fmm_linear_int8")
+@lru_cache(maxsize=None)
+def entry_point(name: str):
+    """A C function by name, for callers that pass addresses themselves (the
+    8-bit operators run between single tokens, where a call's own time counts)."""
+    return getattr(library(), name)
 
 
 def linear_noalloc(scheme: str, A, W, bias, C) -> int:

@@ -70,15 +70,14 @@ def empty_codes(shape: tuple[int, ...], device: torch.device) -> torch.Tensor:
 
 
 # ---------------------------------------------------------------- operands
-class _Rows(NamedTuple):
-    """A tensor as rows: address, count, length and step in elements."""
+# A call between two single tokens is a few microseconds of GPU time, so the
+# checks below read each tensor's attributes once and pass plain integers on.
+_ROW_TYPES = {torch.bfloat16: _native.FMM_DTYPE_BF16, torch.float16: _native.FMM_DTYPE_F16,
+              torch.float32: _native.FMM_DTYPE_F32}
 
-    ptr: int
-    rows: int
-    inner: int
-    pitch: int
-    itemsize: int
-    keep: torch.Tensor  # holds the memory where the rows had to be copied
+
+# A tensor as rows: (address, count, length and step in elements, element size)
+_Rows = tuple[int, int, int, int, int]
 
 
 def _flat(tensor: torch.Tensor) -> tuple[int, int, int] | None:
@@ -86,120 +85,146 @@ def _flat(tensor: torch.Tensor) -> tuple[int, int, int] | None:
     step apart and the last dimension is dense, else None."""
     shape = tensor.shape
     inner = shape[-1]
-    if tensor.ndim == 1:
-        rows, pitch = 1, inner
-    elif tensor.ndim == 2:
-        rows, pitch = shape[0], tensor.stride(0)
-    else:
-        rows, pitch, step = 1, None, None
-        for size, stride in zip(reversed(shape[:-1]), reversed(tensor.stride()[:-1])):
-            if size == 1:
-                continue
-            if pitch is None:
-                pitch = stride
-            elif stride != step:
-                return None
-            rows *= size
-            step = stride * size
+    if inner and tensor.is_contiguous():
+        rows = tensor.numel() // inner
+        # a single row has no second one to reach
+        return rows, inner, inner if rows > 1 else (inner + 15) & -16
+    rows, pitch, step = 1, None, None
+    for size, stride in zip(reversed(shape[:-1]), reversed(tensor.stride()[:-1])):
+        if size == 1:
+            continue
         if pitch is None:
-            pitch = inner
+            pitch = stride
+        elif stride != step:
+            return None
+        rows *= size
+        step = stride * size
     if inner > 1 and tensor.stride(-1) != 1:
         return None
     if rows <= 1:
-        pitch = _round_up(inner, CODE_ALIGNMENT)  # no second row to reach
+        pitch = (inner + 15) & -16
     elif pitch < inner:
         return None
     return rows, inner, pitch
 
 
-def _input_rows(tensor: torch.Tensor) -> _Rows:
+def _input_rows(tensor: torch.Tensor) -> tuple[torch.Tensor, _Rows]:
+    """The rows, and the tensor that holds them (a copy where they had to be made dense)."""
     flat = _flat(tensor)
     if flat is None:
         tensor = tensor.contiguous()
         flat = _flat(tensor)
-    return _Rows(tensor.data_ptr(), *flat, tensor.element_size(), tensor)
+    return tensor, (tensor.data_ptr(), *flat, tensor.element_size())
 
 
-def _output_rows(tensor: torch.Tensor, shape: torch.Size, dtype: torch.dtype, device: torch.device,
-                 name: str) -> _Rows:
+def _output_rows(tensor: torch.Tensor, shape: torch.Size, dtype: torch.dtype, device: int, name: str,
+                 like: _Rows | None = None) -> _Rows:
     if tensor.shape != shape:
         raise ValueError(f"{name} has shape {tuple(tensor.shape)}, expected {tuple(shape)}")
-    if tensor.device != device or tensor.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype} on {device}")
-    _refuse_grad(tensor)
+    if tensor.get_device() != device or tensor.dtype is not dtype:
+        raise ValueError(f"{name} must be {dtype} on cuda:{device}")
+    if like is not None and (rows := _like(tensor, like)) is not None:
+        return rows
     flat = _flat(tensor)
     if flat is None:
         raise ValueError(f"{name} must have dense rows a constant step apart")
-    return _Rows(tensor.data_ptr(), *flat, tensor.element_size(), tensor)
+    return tensor.data_ptr(), *flat, tensor.element_size()
 
 
-def _input_scales(tensor: torch.Tensor, shape: torch.Size, device: torch.device, name: str) -> torch.Tensor:
+def _like(tensor: torch.Tensor, rows: _Rows) -> _Rows | None:
+    """Rows of a dense tensor with the shape of an operand whose rows are known."""
+    if not tensor.is_contiguous():
+        return None
+    _, count, inner, _, _ = rows
+    return tensor.data_ptr(), count, inner, inner if count > 1 else (inner + 15) & -16, tensor.element_size()
+
+
+def _input_scales(tensor: torch.Tensor, shape: torch.Size, device: int, name: str) -> torch.Tensor:
     if tensor.shape != shape:
         raise ValueError(f"{name} has shape {tuple(tensor.shape)}, expected {tuple(shape)}")
-    if tensor.device != device or tensor.dtype != torch.float32:
-        raise ValueError(f"{name} must be float32 on {device}")
-    _refuse_grad(tensor)
-    return tensor.contiguous()
+    if tensor.get_device() != device or tensor.dtype is not torch.float32:
+        raise ValueError(f"{name} must be float32 on cuda:{device}")
+    return tensor if tensor.is_contiguous() else tensor.contiguous()
 
 
-def _output_scales(tensor: torch.Tensor, shape: torch.Size, device: torch.device) -> torch.Tensor:
+def _output_scales(tensor: torch.Tensor, shape: torch.Size, device: int) -> None:
     if tensor.shape != shape:
         raise ValueError(f"scales has shape {tuple(tensor.shape)}, expected {tuple(shape)}")
-    if tensor.device != device or tensor.dtype != torch.float32 or not tensor.is_contiguous():
-        raise ValueError(f"scales must be contiguous float32 on {device}")
-    _refuse_grad(tensor)
-    return tensor
+    if tensor.get_device() != device or tensor.dtype is not torch.float32 or not tensor.is_contiguous():
+        raise ValueError(f"scales must be contiguous float32 on cuda:{device}")
 
 
-def _refuse_grad(tensor: torch.Tensor) -> None:
-    if tensor.requires_grad and torch.is_grad_enabled():
-        raise ValueError("the B200 8-bit operators do not support autograd")
+def _refuse_grad(*tensors: torch.Tensor | None) -> None:
+    if torch.is_grad_enabled():
+        for tensor in tensors:
+            if tensor is not None and tensor.requires_grad:
+                raise ValueError("the B200 8-bit operators do not support autograd")
 
 
-def _require_cuda(tensor: torch.Tensor, name: str) -> None:
-    if tensor.device.type != "cuda":
+def _require_cuda(tensor: torch.Tensor, name: str) -> int:
+    device = tensor.get_device()
+    if device < 0 or not tensor.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
+    return device
 
 
 def _rows_overlap(a: _Rows, b: _Rows) -> bool:
     """Whether two row operands share a byte."""
-    if a.rows == 0 or b.rows == 0:
+    ptr_a, rows_a, inner_a, pitch_a, size_a = a
+    ptr_b, rows_b, inner_b, pitch_b, size_b = b
+    if rows_a == 0 or rows_b == 0:
         return False
-    width_a, width_b = a.inner * a.itemsize, b.inner * b.itemsize
-    step_a, step_b = a.pitch * a.itemsize, b.pitch * b.itemsize
-    if a.ptr >= b.ptr + (b.rows - 1) * step_b + width_b or b.ptr >= a.ptr + (a.rows - 1) * step_a + width_a:
+    width_a, width_b = inner_a * size_a, inner_b * size_b
+    step_a, step_b = pitch_a * size_a, pitch_b * size_b
+    if ptr_a >= ptr_b + (rows_b - 1) * step_b + width_b or ptr_b >= ptr_a + (rows_a - 1) * step_a + width_a:
         return False
-    if a.rows > 1 and b.rows > 1 and step_a == step_b:
+    if rows_a > 1 and rows_b > 1 and step_a == step_b:
         # columns of one buffer: apart if their byte ranges within a step are
-        offset = (b.ptr - a.ptr) % step_a
+        offset = (ptr_b - ptr_a) % step_a
         return offset < width_a or offset + width_b > step_a
     return True
 
 
 def _row_vector(tensor: torch.Tensor) -> _Rows:
     n = tensor.numel()
-    return _Rows(tensor.data_ptr(), 1 if n else 0, n, n, tensor.element_size(), tensor)
+    return tensor.data_ptr(), 1 if n else 0, n, n, tensor.element_size()
 
 
 def _same_rows(a: _Rows, b: _Rows) -> bool:
-    return a.ptr == b.ptr and a.pitch == b.pitch
+    return a[0] == b[0] and a[3] == b[3]
 
 
-def _refuse_overlap(outputs: tuple[_Rows, ...], inputs: tuple[_Rows, ...]) -> None:
+def _all_apart(operands: list[_Rows]) -> bool:
+    """Whether no operand's address range touches another's: the common case, decided by one sort."""
+    operands.sort()
+    reach = 0
+    for ptr, rows, inner, pitch, itemsize in operands:
+        if ptr < reach:
+            return False
+        if rows:
+            reach = ptr + ((rows - 1) * pitch + inner) * itemsize
+    return True
+
+
+def _refuse_overlap(outputs: list[_Rows], inputs: list[_Rows]) -> None:
+    if _all_apart(outputs + inputs):
+        return
     for i, out in enumerate(outputs):
         for other in outputs[i + 1:] + inputs:
             if _rows_overlap(out, other):
                 raise ValueError("output storage must not overlap inputs or other outputs")
 
 
-def _launch(device: torch.device, function, *args) -> None:
-    """Call ``function`` with ``device`` current, on its current stream."""
-    index = device.index
-    if index == torch.cuda.current_device():
-        function(*args, torch._C._cuda_getCurrentRawStream(index))
-        return
-    with torch.cuda.device(index):
-        function(*args, torch._C._cuda_getCurrentRawStream(index))
+def _launch(device: int, name: str, *args) -> None:
+    """Call the C entry point with ``device`` current, on its current stream."""
+    function = _native.entry_point(name)
+    if device == torch._C._cuda_getDevice():
+        code = function(*args, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            code = function(*args, torch._C._cuda_getCurrentRawStream(device))
+    if code:
+        _native.check(code, name)
 
 
 # ---------------------------------------------------------------- operators
@@ -211,20 +236,27 @@ def quantize_rows(x: torch.Tensor, *, codes: torch.Tensor | None = None,
     with ``a`` the row's largest magnitude.  A row of zeros has scale 0; a row
     with an infinity or a NaN has codes 0 and scale NaN.  ``codes`` and
     ``scales`` are written and returned where given."""
-    _require_cuda(x, "x")
-    dtype = _native.row_dtype_id(x.dtype)
-    if x.ndim < 1 or x.shape[-1] < 1:
+    device = _require_cuda(x, "x")
+    dtype = _ROW_TYPES.get(x.dtype)
+    if dtype is None:
+        raise ValueError(f"the 8-bit operators take BF16, FP16 or FP32 rows, not {x.dtype}")
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] < 1:
         raise ValueError("x must have a last dimension of at least one element")
-    _refuse_grad(x)
-    source = _input_rows(x)
-    codes = empty_codes(x.shape, x.device) if codes is None else codes
-    scales = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32) if scales is None else scales
-    q = _output_rows(codes, x.shape, torch.int8, x.device, "codes")
-    _output_scales(scales, x.shape[:-1], x.device)
-    _refuse_overlap((q, _row_vector(scales)), (source,))
-    if source.rows:
-        _launch(x.device, _native.quantize_rows, dtype, source.ptr, source.rows, source.inner, source.pitch, q.ptr,
-                q.pitch, scales.data_ptr())
+    _refuse_grad(x, codes, scales)
+    held, source = _input_rows(x)
+    leading = shape[:-1]
+    if codes is None:
+        codes = empty_codes(shape, x.device)
+    if scales is None:
+        scales = torch.empty(leading, device=x.device, dtype=torch.float32)
+    q = _output_rows(codes, shape, torch.int8, device, "codes", source)
+    _output_scales(scales, leading, device)
+    rows = source[1]
+    s = scales.data_ptr(), 1 if rows else 0, rows, rows, 4
+    _refuse_overlap([q, s], [source])
+    if rows:
+        _launch(device, "fmm_quantize_rows", dtype, *source[:4], q[0], q[3], s[0])
     return Int8Rows(codes, scales)
 
 
@@ -238,49 +270,59 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
     is quantised unrounded as by ``quantize_rows``.  ``weight[K]`` has ``x``'s
     type or FP32.  ``residual_out`` may be ``residual`` or ``x`` itself, which
     updates the stream in place."""
-    _require_cuda(x, "x")
-    if x.dtype not in _HALF_TYPES:
-        raise ValueError(f"rms_norm_int8 takes BF16 or FP16 rows, not {x.dtype}")
-    if x.ndim < 1 or x.shape[-1] < 1:
+    device = _require_cuda(x, "x")
+    kind = x.dtype
+    if kind not in _HALF_TYPES:
+        raise ValueError(f"rms_norm_int8 takes BF16 or FP16 rows, not {kind}")
+    shape = x.shape
+    if len(shape) < 1 or shape[-1] < 1:
         raise ValueError("x must have a last dimension of at least one element")
-    if weight.shape != x.shape[-1:]:
-        raise ValueError(f"weight has shape {tuple(weight.shape)}, expected {tuple(x.shape[-1:])}")
-    if weight.device != x.device or weight.dtype not in (x.dtype, torch.float32):
+    if weight.shape != shape[-1:]:
+        raise ValueError(f"weight has shape {tuple(weight.shape)}, expected {tuple(shape[-1:])}")
+    gain_kind = weight.dtype
+    if weight.get_device() != device or (gain_kind is not kind and gain_kind is not torch.float32):
         raise ValueError("weight must have x's dtype or float32, on x's device")
     if not 0.0 <= eps < float("inf"):
         raise ValueError("eps must be finite and not negative")
     if residual is None and residual_out is not None:
         raise ValueError("residual_out needs a residual")
-    _refuse_grad(x)
-    _refuse_grad(weight)
-    source = _input_rows(x)
-    gain = _row_vector(weight.contiguous())
-    inputs = [source, gain]
-    codes = empty_codes(x.shape, x.device) if codes is None else codes
-    scales = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32) if scales is None else scales
-    q = _output_rows(codes, x.shape, torch.int8, x.device, "codes")
-    _output_scales(scales, x.shape[:-1], x.device)
-    outputs = [q, _row_vector(scales)]
-    added, stream_out = None, None
-    if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != x.device:
-            raise ValueError("residual must have x's shape, dtype and device")
-        _refuse_grad(residual)
-        added = _input_rows(residual)
-        if residual_out is None:
-            residual_out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-        stream_out = _output_rows(residual_out, x.shape, x.dtype, x.device, "residual_out")
+    _refuse_grad(x, weight, residual, codes, scales, residual_out)
+    held, source = _input_rows(x)
+    if not weight.is_contiguous():
+        weight = weight.contiguous()
+    ptr, rows, inner, pitch, _ = source
+    gain = weight.data_ptr(), 1, inner, inner, 4 if gain_kind is torch.float32 else 2
+    leading = shape[:-1]
+    if codes is None:
+        codes = empty_codes(shape, x.device)
+    if scales is None:
+        scales = torch.empty(leading, device=x.device, dtype=torch.float32)
+    q = _output_rows(codes, shape, torch.int8, device, "codes", source)
+    _output_scales(scales, leading, device)
+    s = scales.data_ptr(), 1 if rows else 0, rows, rows, 4
+    if residual is None:
+        _refuse_overlap([q, s], [source, gain])
+        if rows:
+            _launch(device, "fmm_rms_norm_int8", _ROW_TYPES[kind], _ROW_TYPES[gain_kind], ptr, pitch, None, 0, gain[0],
+                    rows, inner, eps, None, 0, q[0], q[3], s[0])
+        return NormedInt8Rows(codes, scales, None)
+    if residual.shape != shape or residual.dtype is not kind or residual.get_device() != device:
+        raise ValueError("residual must have x's shape, dtype and device")
+    held_residual, added = residual, _like(residual, source)
+    if added is None:
+        held_residual, added = _input_rows(residual)
+    if residual_out is None:
+        residual_out = torch.empty(shape, device=x.device, dtype=kind)
+    stream = _output_rows(residual_out, shape, kind, device, "residual_out", source)
+    if not _all_apart([q, s, stream, source, gain, added]):
         for other in (source, added):
-            if not _same_rows(stream_out, other) and _rows_overlap(stream_out, other):
+            if not _same_rows(stream, other) and _rows_overlap(stream, other):
                 raise ValueError("residual_out must be residual, x or storage of its own")
-        _refuse_overlap((stream_out,), (gain, *outputs))
-        inputs.append(added)
-    _refuse_overlap(tuple(outputs), tuple(inputs))
-    if source.rows:
-        _launch(x.device, _native.rms_norm_int8, _native.row_dtype_id(x.dtype), _native.row_dtype_id(weight.dtype),
-                source.ptr, source.pitch, None if added is None else added.ptr, 0 if added is None else added.pitch,
-                gain.ptr, source.rows, source.inner, eps, None if stream_out is None else stream_out.ptr,
-                0 if stream_out is None else stream_out.pitch, q.ptr, q.pitch, scales.data_ptr())
+        _refuse_overlap([stream], [gain, q, s])
+        _refuse_overlap([q, s], [source, gain, added])
+    if rows:
+        _launch(device, "fmm_rms_norm_int8", _ROW_TYPES[kind], _ROW_TYPES[gain_kind], ptr, pitch, added[0], added[3],
+                gain[0], rows, inner, eps, stream[0], stream[3], q[0], q[3], s[0])
     return NormedInt8Rows(codes, scales, residual_out)
 
 
@@ -295,13 +337,14 @@ def linear_int8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.T
     exactly in 32-bit integers (``K`` up to 131071), scaled and biased in FP32
     and rounded once.  Code rows must start on 16-byte boundaries, as
     ``quantize_rows``, ``rms_norm_int8`` and ``empty_codes`` make them."""
-    _require_cuda(codes, "codes")
-    device = codes.device
-    if codes.dtype != torch.int8 or weight_codes.dtype != torch.int8 or weight_codes.device != device:
+    device = _require_cuda(codes, "codes")
+    if (codes.dtype is not torch.int8 or weight_codes.dtype is not torch.int8
+            or weight_codes.get_device() != device):
         raise ValueError("codes and weight_codes must be int8 tensors of one device")
-    if codes.ndim < 1 or weight_codes.ndim != 2 or codes.shape[-1] != weight_codes.shape[1]:
+    token_shape, weight_shape = codes.shape, weight_codes.shape
+    if len(token_shape) < 1 or len(weight_shape) != 2 or token_shape[-1] != weight_shape[1]:
         raise ValueError("codes and weight_codes shapes do not form a linear")
-    columns, inner = weight_codes.shape
+    columns, inner = weight_shape
     if columns < 1 or inner < 1:
         raise ValueError("matrix dimensions must be positive")
     if inner > MAX_INNER:
@@ -310,32 +353,36 @@ def linear_int8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.T
         dtype = out.dtype if out is not None else bias.dtype if bias is not None else torch.bfloat16
     if dtype not in _HALF_TYPES:
         raise ValueError(f"linear_int8 writes BF16 or FP16, not {dtype}")
+    _refuse_grad(scales, weight_scales, bias, out)
     q, w = _flat(codes), _flat(weight_codes)
     if q is None or w is None:
         raise ValueError("codes must have dense rows a constant step apart")
-    token_scales = _input_scales(scales, codes.shape[:-1], device, "scales")
-    channel_scales = _input_scales(weight_scales, weight_codes.shape[:1], device, "weight_scales")
+    leading = token_shape[:-1]
+    scales = _input_scales(scales, leading, device, "scales")
+    weight_scales = _input_scales(weight_scales, weight_shape[:1], device, "weight_scales")
     if bias is not None:
-        if bias.shape != (columns,) or bias.dtype != dtype or bias.device != device:
+        if bias.shape != weight_shape[:1] or bias.dtype is not dtype or bias.get_device() != device:
             raise ValueError(f"bias must be {dtype} [N] on the codes' device")
-        _refuse_grad(bias)
-        bias = bias.contiguous()
-    shape = torch.Size((*codes.shape[:-1], columns))
-    fresh = out is None
-    if fresh:
-        out = torch.empty(shape, device=device, dtype=dtype)
-    result = _output_rows(out, shape, dtype, device, "out")
+        if not bias.is_contiguous():
+            bias = bias.contiguous()
     rows, _, pitch = q
-    if not fresh:
-        inputs = [_Rows(codes.data_ptr(), *q, 1, codes), _Rows(weight_codes.data_ptr(), *w, 1, weight_codes),
-                  _row_vector(token_scales), _row_vector(channel_scales)]
-        if bias is not None:
-            inputs.append(_row_vector(bias))
-        _refuse_overlap((result,), tuple(inputs))
+    ptr, weight_ptr, bias_ptr = codes.data_ptr(), weight_codes.data_ptr(), None if bias is None else bias.data_ptr()
+    scales_ptr, weight_scales_ptr = scales.data_ptr(), weight_scales.data_ptr()
+    if out is None:
+        out = torch.empty((*leading, columns), device=codes.device, dtype=dtype)
+        result_ptr, result_pitch = out.data_ptr(), columns if rows > 1 else (columns + 15) & -16
+    else:
+        result = _output_rows(out, torch.Size((*leading, columns)), dtype, device, "out")
+        result_ptr, result_pitch = result[0], result[3]
+        inputs = [(ptr, *q, 1), (weight_ptr, *w, 1), (scales_ptr, 1, rows, rows, 4),
+                  (weight_scales_ptr, 1, columns, columns, 4)]
+        if bias_ptr is not None:
+            inputs.append((bias_ptr, 1, columns, columns, 2))
+        if rows and not _all_apart([result, *inputs]):
+            _refuse_overlap([result], inputs)
     if rows:
-        _launch(device, _native.linear_int8, _native.row_dtype_id(dtype), codes.data_ptr(), pitch,
-                token_scales.data_ptr(), weight_codes.data_ptr(), w[2], channel_scales.data_ptr(),
-                None if bias is None else bias.data_ptr(), result.ptr, result.pitch, rows, inner, columns)
+        _launch(device, "fmm_linear_int8", _ROW_TYPES[dtype], ptr, pitch, scales_ptr, weight_ptr, w[2],
+                weight_scales_ptr, bias_ptr, result_ptr, result_pitch, rows, inner, columns)
     return out
 
 
@@ -463,7 +510,7 @@ class Int8Plan:
     def _refuse_weight(workspace: Int8Workspace, weight: Int8PackedWeight) -> None:
         for buffer in (workspace.codes, workspace.scales):
             for packed in (weight.codes, weight.scales):
-                if _rows_overlap(_input_rows(buffer), _input_rows(packed)):
+                if _rows_overlap(_input_rows(buffer)[1], _input_rows(packed)[1]):
                     raise ValueError("work buffers must not overlap")
 
     @staticmethod
@@ -471,9 +518,9 @@ class Int8Plan:
         """What the first kernel reads or writes must outlive the second's output."""
         if output is None or _flat(output) is None:
             return  # a malformed output is refused where it is used
-        rows = _input_rows(output)
+        rows = _input_rows(output)[1]
         for tensor in tensors:
-            if tensor is not None and _rows_overlap(rows, _input_rows(tensor)):
+            if tensor is not None and _rows_overlap(rows, _input_rows(tensor)[1]):
                 raise ValueError("output storage must not overlap inputs or workspace")
 
 

@@ -8,7 +8,7 @@ import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 from rdna3_fastmm import _native, int8
-from rdna3_fastmm.int8 import _flat, _row_vector, _Rows, _rows_overlap
+from rdna3_fastmm.int8 import _flat, _row_vector, _rows_overlap
 
 P = ctypes.c_void_p
 FAKE, ODD = P(0x10000), P(0x10001)
@@ -70,8 +70,6 @@ def test_linear_int8_refusals(change, code):
 def test_refusals_reach_python_as_value_errors():
     with pytest.raises(ValueError, match="16-byte"):
         _native.check(_linear(codes=ODD), "fmm_linear_int8")
-    with pytest.raises(ValueError, match="not torch.float64"):
-        _native.row_dtype_id(torch.float64)
 
 
 def test_rows_of_views():
@@ -91,7 +89,7 @@ def test_rows_of_views():
 
 def _cut(buffer, first, width):
     part = buffer[:, first:first + width]
-    return _Rows(part.data_ptr(), *_flat(part), part.element_size(), part)
+    return part.data_ptr(), *_flat(part), part.element_size()
 
 
 def test_overlap_of_rows():
@@ -105,6 +103,18 @@ def test_overlap_of_rows():
     assert not _rows_overlap(_cut(buffer[:2], 0, 100), _cut(buffer[2:], 0, 100))
     assert _rows_overlap(_row_vector(buffer.view(-1)[150:160]), _cut(buffer, 0, 50))
     assert not _rows_overlap(_row_vector(buffer.view(-1)[:0]), _cut(buffer, 0, 50))
+
+
+def test_operands_apart_by_one_sort():
+    buffer = torch.zeros((4, 100), dtype=torch.int16)
+    apart = int8._all_apart
+    assert apart([_cut(buffer[2:], 0, 100), _cut(buffer[:2], 0, 100)])
+    assert apart([_cut(buffer[:2], 0, 100), _row_vector(buffer.view(-1)[200:]), _row_vector(buffer.view(-1)[:0])])
+    assert not apart([_cut(buffer, 0, 50), _cut(buffer, 50, 50)])  # beside each other: for the closer look
+    assert not apart([_cut(buffer[:3], 0, 100), _row_vector(buffer.view(-1)[299:])])
+    int8._refuse_overlap([_cut(buffer, 0, 50)], [_cut(buffer, 50, 50)])
+    with pytest.raises(ValueError, match="overlap"):
+        int8._refuse_overlap([_cut(buffer, 0, 50)], [_cut(buffer, 49, 50)])
 
 
 def test_cpu_tensors_and_plans_are_refused():
