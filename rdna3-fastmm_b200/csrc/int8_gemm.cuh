@@ -23,7 +23,8 @@ namespace fmm {
 
 constexpr int kI8TileN = 128;    // output channels of an SM's tile
 constexpr int kI8BlockK = 128;   // k of one 128-byte swizzle row
-constexpr int kI8Threads = 192;
+constexpr int kI8EpilogueWarps = 8;  // two for each 32 TMEM lanes, every other 32 columns each
+constexpr int kI8Threads = 64 + 32 * kI8EpilogueWarps;
 constexpr int kI8MaxStages = 24;
 
 struct Int8LinearParams {
@@ -155,8 +156,10 @@ __device__ __forceinline__ void store_columns(const Int8LinearParams& p, const u
 //   warp 0      TMA producer: a rows x 128 box of W and a tok x 128 box of Q a
 //               stage (128-byte swizzle; what lies outside reads as zero).
 //   warp 1      MMA issuer: 4 x m128 n<tok> k32 a stage; owns TMEM.
-//   warps 2..5  epilogue: tcgen05.ld 32 lanes x 32 columns, scale, bias, one
-//               rounding, 64-byte row segments.
+//   warps 2..9  epilogue: tcgen05.ld 32 lanes x 32 columns, scale, bias, one
+//               rounding, 64-byte row segments.  Eight warps, because one to
+//               a scheduler waits for its own results (20000 x 256 x 1000:
+//               35 us with four).
 // A tile may have fewer than 128 channels, so that a few tokens' tiles, which
 // cost the weight's bytes and little else, come out even over the SMs; the
 // product runs over 128 rows of shared memory all the same and the sums of the
@@ -228,7 +231,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(tfull_bar + 8 * b, 1);
-      mbar_init(tempty_bar + 8 * b, 4);  // one arrival per epilogue warp
+      mbar_init(tempty_bar + 8 * b, kI8EpilogueWarps);  // one arrival each
     }
     mbar_init(drain_bar, 1);
     *abort = 0;
@@ -314,6 +317,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     }
   } else {
     const int quarter = warp & 3;  // TMEM lanes this warp may access
+    const int first = (warp - 2) / 4 * 32;
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int t = blockIdx.x; t < total; t += gridDim.x) {
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       const int tokens = static_cast<int>(p.M - m0 < p.tok ? p.M - m0 : p.tok);
       const float channel_scale = n < p.N ? p.channel_scales[n] : 0.0f;
       const float bias = n < p.N ? load_bias<kBf16>(p.bias, n) : 0.0f;
-      float token_scale = lane < tokens ? p.token_scales[m0 + lane] : 0.0f;
+      float token_scale = first + lane < tokens ? p.token_scales[m0 + first + lane] : 0.0f;
       int ready = 0;
       if (lane == 0) ready = mbar_wait_bounded(tfull_bar + 8 * acc, acc_phase, abort, p.timeout_ns, 24) ? 1 : 0;
       ready = __shfl_sync(0xffffffffu, ready, 0);
@@ -335,11 +339,11 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * p.tmem_cols;
       if (quarter * 32 < p.rows) {
 #pragma unroll 1
-        for (int c = 0; c < tokens; c += 32) {
+        for (int c = first; c < tokens; c += 64) {
           uint32_t v[32];
           tc_ld_32x32b_x32(t_addr + c, v);
           // the next columns' scales, before they are waited for
-          const int next = c + 32 + lane;
+          const int next = c + 64 + lane;
           const float next_scale = next < tokens ? p.token_scales[m0 + next] : 0.0f;
           tc_wait_ld();
           store_columns<kBf16>(p, v, m0, c, tokens, n, token_scale, channel_scale, bias);
@@ -412,7 +416,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(tfull_bar + 8 * b, 1);
-      mbar_init(tempty_bar + 8 * b, 8);  // 4 epilogue warps x 2 CTAs
+      mbar_init(tempty_bar + 8 * b, 2 * kI8EpilogueWarps);  // of both CTAs
     }
     mbar_init(drain_bar, 1);
     *abort = 0;
@@ -542,6 +546,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     }
   } else {
     const int quarter = warp & 3;
+    const int first = (warp - 2) / 4 * 32;
     const uint32_t tempty_even = map_to_cta(tempty_bar, 0);
     int acc = 0;
     uint32_t acc_phase = 0;
@@ -553,7 +558,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       const int tokens = static_cast<int>(p.M - m0 < Cfg::kTile ? p.M - m0 : Cfg::kTile);
       const float channel_scale = n < p.N ? p.channel_scales[n] : 0.0f;
       const float bias = n < p.N ? load_bias<kBf16>(p.bias, n) : 0.0f;
-      float token_scale = lane < tokens ? p.token_scales[m0 + lane] : 0.0f;
+      float token_scale = first + lane < tokens ? p.token_scales[m0 + first + lane] : 0.0f;
       int ready = 0;
       if (lane == 0)
         ready = mbar_wait_bounded_cluster(tfull_bar + 8 * acc, acc_phase, abort, p.timeout_ns, 44) ? 1 : 0;
@@ -563,10 +568,10 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       const uint32_t t_addr =
           tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * Cfg::kTile);
 #pragma unroll 1
-      for (int c = 0; c < tokens; c += 32) {
+      for (int c = first; c < tokens; c += 64) {
         uint32_t v[32];
         tc_ld_32x32b_x32(t_addr + c, v);
-        const int next = c + 32 + lane;
+        const int next = c + 64 + lane;
         const float next_scale = next < tokens ? p.token_scales[m0 + next] : 0.0f;
         tc_wait_ld();
         store_columns<kBf16>(p, v, m0, c, tokens, n, token_scale, channel_scale, bias);
