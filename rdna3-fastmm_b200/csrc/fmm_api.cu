@@ -1156,79 +1156,121 @@ int codes_map(CUtensorMap* map, const void* base, int64_t k, int64_t rows, int64
 
 constexpr size_t kI8MaxSmem = 232448;
 
-// How int8_linear_kernel takes a product: channels and tokens of a tile.
+// Y[M][N] (16-bit) as a 2-D map over (channel, token); box 32 x 32, 64-byte swizzle.
+int output_map(CUtensorMap* map, void* base, int64_t M, int64_t N, int64_t ld) {
+  PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
+  if (int rc = tensor_map_encoder(&encode)) return rc;
+  cuuint64_t dims[2] = {static_cast<cuuint64_t>(N), static_cast<cuuint64_t>(M)};
+  cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld * 2)};
+  cuuint32_t box[2] = {32, 32};
+  cuuint32_t elem[2] = {1, 1};
+  CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, base, dims, strides, box, elem,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FMM_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string(r) + ")");
+  return FMM_OK;
+}
+
+// How a product is taken: which way the tiles lie (two SMs a tile: channels in
+// the lanes; with tokens there its outputs were no faster, 65536 x 4608 x 12288
+// 2.54 ms to 2.24), two SMs a tile or one, and an SM's tile.
 struct Int8Shape {
-  int rows, tok;
+  bool tokens, pair;
+  int lanes, cols;
 };
 
-// Measured (one B200, us a 128-deep column of K): a tile of 128 channels costs
-// 0.15 + 0.0011 tok (tok = 64, 128, 192, 256: 0.20, 0.28, 0.36, 0.43), one of 64
-// channels about an eighth less, a 256 x 256 tile of two SMs 0.37 however
-// many of its tokens exist; every launch some 4 more.  The estimates pick the
-// least whole waves of tiles.
-double int8_single_cost(int64_t M, int64_t K, int64_t N, const Int8Shape& s, int sms) {
-  const int64_t tiles = ceil_div(M, s.tok) * ceil_div(N, s.rows);
-  const double column = (0.15 + 0.0011 * s.tok) * (s.rows < kI8TileN ? 0.875 : 1.0);
-  return 4.0 + double(ceil_div(tiles, sms)) * double(ceil_div(K, kI8BlockK)) * column;
-}
-double int8_pair_cost(int64_t M, int64_t K, int64_t N, int sms) {
-  const int64_t tiles = ceil_div(M, 256) * ceil_div(N, 256);
-  return 5.0 + double(ceil_div(tiles, sms / 2)) * double(ceil_div(K, kI8BlockK)) * 0.37;
+// Measured (one B200, us): a 128-deep column of K costs a tile of 128 lanes
+// 0.15 + 0.0011 cols (64, 128, 192, 256: 0.20, 0.28, 0.36, 0.43), one of 64 lanes
+// about an eighth less, a 256 x 256 tile of two SMs 0.37 however many of its
+// columns exist.  The outputs of an SM's tile take 0.5 + 0.0097 cols beside the
+// next tile's products, 0.0076 by TMA; every launch costs some 4 more.
+double int8_cost(int64_t M, int64_t K, int64_t N, const Int8Shape& s, int sms) {
+  const int64_t lane_end = s.tokens ? M : N, col_end = s.tokens ? N : M;
+  const double columns = double(ceil_div(K, kI8BlockK));
+  const double out = 0.5 + (s.tokens ? 0.0076 : 0.0097) * s.cols;
+  double tile = 0;
+  int64_t tiles = 0, units = 0;
+  if (s.pair) {
+    tiles = ceil_div(lane_end, 256) * ceil_div(col_end, 256);
+    units = sms / 2;
+    tile = columns * 0.37;
+  } else {
+    tiles = ceil_div(lane_end, s.lanes) * ceil_div(col_end, s.cols);
+    units = sms;
+    tile = columns * (0.15 + 0.0011 * s.cols) * (s.lanes < kI8Lanes ? 0.875 : 1.0);
+  }
+  return (s.pair ? 5.0 : 4.0) + double(ceil_div(tiles, units)) * (tile > out ? tile : out);
 }
 
-Int8Shape choose_int8_shape(int64_t M, int64_t K, int64_t N, int sms, double* cost) {
-  Int8Shape best = {kI8TileN, 16};
-  *cost = 1e30;
-  auto consider = [&](int64_t tok) {
-    for (int rows : {kI8TileN, kI8TileN / 2}) {
-      const Int8Shape s = {rows, static_cast<int>(tok)};
-      const double c = int8_single_cost(M, K, N, s, sms);
-      if (c < *cost) {
-        *cost = c;
-        best = s;
-      }
+// The least estimate over tokens in equal tiles and tiles of the usual widths;
+// `aligned`: the outputs may leave by TMA.
+Int8Shape choose_int8_shape(int64_t M, int64_t K, int64_t N, bool aligned, int sms) {
+  Int8Shape best = {false, false, kI8Lanes, 16};
+  double least = 1e30;
+  auto consider = [&](bool tokens, bool pair, int lanes, int64_t cols) {
+    const Int8Shape s = {tokens, pair, lanes, static_cast<int>(cols)};
+    const double c = int8_cost(M, K, N, s, sms);
+    if (c < least) {
+      least = c;
+      best = s;
     }
   };
-  // the tokens in equal tiles, and the widths that tiles of many tokens have
-  for (int64_t pieces = ceil_div(M, 256); pieces <= 16; ++pieces) consider(round_up(ceil_div(M, pieces), 16));
-  if (M > 256)
-    for (int64_t tok : {64, 96, 128, 192, 256}) consider(tok);
+  for (int lanes : {kI8Lanes, kI8Lanes / 2}) {
+    for (int64_t pieces = ceil_div(M, 256); pieces <= 16; ++pieces)
+      consider(false, false, lanes, round_up(ceil_div(M, pieces), 16));
+    if (M > 256)
+      for (int64_t tok : {64, 96, 128, 192, 256}) consider(false, false, lanes, tok);
+  }
+  consider(false, true, kI8Lanes, 256);
+  if (aligned && M > 64) {
+    for (int64_t cols : {64, 96, 128, 192, 256}) consider(true, false, kI8Lanes, cols);
+  }
   return best;
 }
 
-template <bool kBf16>
+template <bool kBf16, bool kTokens>
 int launch_int8_single(const int8_t* codes, int64_t ldq, const int8_t* weight_codes, int64_t ldw, Int8LinearParams p,
                        const Int8Shape& shape, int sms, cudaStream_t stream) {
   static bool configured[kMaxDevices] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
-  p.rows = shape.rows;
-  p.tok = shape.tok;
+  p.lanes = shape.lanes;
+  p.cols = shape.cols;
   p.tmem_cols = 32;
-  while (p.tmem_cols < static_cast<uint32_t>(p.tok)) p.tmem_cols *= 2;
-  p.tiles_m = static_cast<int32_t>(ceil_div(p.M, p.tok));
-  p.tiles_n = static_cast<int32_t>(ceil_div(p.N, p.rows));
+  while (p.tmem_cols < static_cast<uint32_t>(p.cols)) p.tmem_cols *= 2;
+  p.tiles_m = static_cast<int32_t>(ceil_div(p.M, kTokens ? p.lanes : p.cols));
+  p.tiles_n = static_cast<int32_t>(ceil_div(p.N, kTokens ? p.cols : p.lanes));
   // 128-deep columns of a stage: as many as keep it at 64 KB (three stages), up
   // to four.  64 channels x 16 tokens, K = 4096, with 1, 2, 4: 13.4, 10.7, 10.0
   // us; 128 x 128: 14.3, 13.5; 128 x 192 with 1, 2: 27.1, 32.8
-  p.atoms = p.rows + p.tok <= 128 ? 4 : p.rows + p.tok <= 256 ? 2 : 1;
-  const size_t stage = p.atoms * size_t(p.rows + p.tok) * kI8BlockK;
-  // alignment, barriers, and the rows that products read behind the last stage's
-  const size_t control = 1024 + 8 * (2 * kI8MaxStages + 6) + size_t(kI8TileN - p.rows) * kI8BlockK;
+  p.atoms = p.lanes + p.cols <= 128 ? 4 : p.lanes + p.cols <= 256 ? 2 : 1;
+  const size_t stage = p.atoms * size_t(p.lanes + p.cols) * kI8BlockK;
+  // alignment, barriers, blocks of outputs, and the rows that products read
+  // behind the last stage's
+  const size_t control = 1024 + 8 * (2 * kI8MaxStages + 6) + size_t(kI8Lanes - p.lanes) * kI8BlockK +
+                         (kTokens ? size_t(kI8EpilogueWarps) * 2 * kI8BlockBytes : 0);
   p.stages = kI8MaxStages;
   while (p.stages > 1 && p.stages * stage + control > kI8MaxSmem) --p.stages;
   const size_t smem = p.stages * stage + control;
-  CUtensorMap map_w, map_q;
-  if (int rc = codes_map(&map_w, weight_codes, p.K, p.N, ldw, static_cast<uint32_t>(p.rows))) return rc;
-  if (int rc = codes_map(&map_q, codes, p.K, p.M, ldq, static_cast<uint32_t>(p.tok))) return rc;
+  CUtensorMap map_a, map_b;
+  if (int rc = codes_map(&map_a, kTokens ? codes : weight_codes, p.K, kTokens ? p.M : p.N, kTokens ? ldq : ldw,
+                         static_cast<uint32_t>(p.lanes)))
+    return rc;
+  if (int rc = codes_map(&map_b, kTokens ? weight_codes : codes, p.K, kTokens ? p.N : p.M, kTokens ? ldw : ldq,
+                         static_cast<uint32_t>(p.cols)))
+    return rc;
+  CUtensorMap map_c = map_a;  // not read where tokens are columns
+  if (kTokens) {
+    if (int rc = output_map(&map_c, p.out, p.M, p.N, p.ldc)) return rc;
+  }
   {
     std::lock_guard<std::mutex> lock(g_device_mutex);
-    if (int rc = ensure_smem_attribute(configured[dev], int8_linear_kernel<kBf16>, kI8MaxSmem)) return rc;
+    if (int rc = ensure_smem_attribute(configured[dev], int8_linear_kernel<kBf16, kTokens>, kI8MaxSmem)) return rc;
   }
   const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n;
   const int grid = static_cast<int>(tiles < sms ? tiles : sms);
-  int8_linear_kernel<kBf16><<<grid, kI8Threads, smem, stream>>>(map_w, map_q, p);
+  int8_linear_kernel<kBf16, kTokens><<<grid, kI8Threads, smem, stream>>>(map_a, map_b, map_c, p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return cuda_fail(e, "8-bit linear launch");
   return FMM_OK;
@@ -1244,10 +1286,10 @@ int launch_int8_pair(const int8_t* codes, int64_t ldq, const int8_t* weight_code
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
   p.tiles_m = static_cast<int32_t>(ceil_div(p.M, Cfg::kTile));
   p.tiles_n = static_cast<int32_t>(ceil_div(p.N, Cfg::kTile));
-  CUtensorMap map_w, map_q, map_q16;
-  if (int rc = codes_map(&map_w, weight_codes, p.K, p.N, ldw, 128)) return rc;
-  if (int rc = codes_map(&map_q, codes, p.K, p.M, ldq, 128)) return rc;
-  if (int rc = codes_map(&map_q16, codes, p.K, p.M, ldq, 16)) return rc;
+  CUtensorMap map_a, map_b, map_b16;
+  if (int rc = codes_map(&map_a, weight_codes, p.K, p.N, ldw, 128)) return rc;
+  if (int rc = codes_map(&map_b, codes, p.K, p.M, ldq, 128)) return rc;
+  if (int rc = codes_map(&map_b16, codes, p.K, p.M, ldq, 16)) return rc;
   {
     std::lock_guard<std::mutex> lock(g_device_mutex);
     if (int rc = ensure_smem_attribute(configured[dev], int8_linear_pair_kernel<kBf16>, Cfg::kSmemBytes)) return rc;
@@ -1266,7 +1308,7 @@ int launch_int8_pair(const int8_t* codes, int64_t ldq, const int8_t* weight_code
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, int8_linear_pair_kernel<kBf16>, map_w, map_q, map_q16, p);
+  e = cudaLaunchKernelEx(&cfg, int8_linear_pair_kernel<kBf16>, map_a, map_b, map_b16, p);
   if (e != cudaSuccess) return cuda_fail(e, "8-bit linear (pair) launch");
   return FMM_OK;
 }
@@ -1342,7 +1384,7 @@ int launch_linear_int8(const int8_t* codes, int64_t ldq, const int8_t* weight_co
   const int sms = usable_sms(info);
   p.group_m = 16;
   p.timeout_ns = g_timeout_ns;
-  if (ceil_div(p.M, 16) * ceil_div(p.N, kI8TileN / 2) > (int64_t(1) << 30))
+  if (ceil_div(p.M, 16) * ceil_div(p.N, 64) > (int64_t(1) << 30))
     return fail(FMM_ERR_TOO_LARGE, "too many tiles");
   const int channels = int8_few_channels(p.N, sms);
   if ((p.M <= 2 || (p.M <= 4 && channels < 4)) && int8_few_fits(p.M, p.K)) {
@@ -1364,11 +1406,11 @@ int launch_linear_int8(const int8_t* codes, int64_t ldq, const int8_t* weight_co
     if (p.M == 2) return launch_int8_few_tokens<kBf16, 2>(f, channels, sms, stream);
     return launch_int8_few_tokens<kBf16, 4>(f, channels, sms, stream);
   }
-  double cost = 0;
-  const Int8Shape shape = choose_int8_shape(p.M, p.K, p.N, sms, &cost);
-  if (int8_pair_cost(p.M, p.K, p.N, sms) < cost)
-    return launch_int8_pair<kBf16>(codes, ldq, weight_codes, ldw, p, sms, stream);
-  return launch_int8_single<kBf16>(codes, ldq, weight_codes, ldw, p, shape, sms, stream);
+  const bool rows16 = aligned(p.out, 16) && p.ldc % 8 == 0;
+  const Int8Shape shape = choose_int8_shape(p.M, p.K, p.N, rows16, sms);
+  if (shape.pair) return launch_int8_pair<kBf16>(codes, ldq, weight_codes, ldw, p, sms, stream);
+  return shape.tokens ? launch_int8_single<kBf16, true>(codes, ldq, weight_codes, ldw, p, shape, sms, stream)
+                      : launch_int8_single<kBf16, false>(codes, ldq, weight_codes, ldw, p, shape, sms, stream);
 }
 
 // Device address of g_noalloc_scratch on the current device.  In host code the

@@ -3,15 +3,17 @@
 // the sum in 32-bit integers on the 5th-generation tensor cores
 // (tcgen05.mma.kind::i8), so it is exact for K <= 131071.
 //
-// Tiles are transposed: the MMA's 128 rows (TMEM lanes) are output channels
-// and its columns are tokens.  A few tokens then cost a few columns instead of
-// a padded 128-row tile, t[n] and b[n] are one register a lane, and a warp
-// writes 32 consecutive outputs of one token, whatever N, ldc or the alignment
-// of Y (no vector store to fall back from).
+// Tiles lie one of two ways.  With channels in the MMA's rows (TMEM lanes) and
+// tokens in its columns, a few tokens cost a few columns instead of a padded
+// 128-row tile, t[n] and b[n] are one register a lane, and a warp writes 32
+// consecutive outputs of one token, whatever N, ldc or the alignment of Y.
+// With tokens in the rows (kTokens) a lane holds 32 consecutive outputs of a
+// token, which leave by TMA stores; that needs rows of Y on 16-byte boundaries
+// and pays where many outputs meet a short K (50000 x 64 x 304: 31 us, 17).
 //
 // Three kernels:
 //   int8_linear_few_kernel   a few tokens: bound by reading the weight
-//   int8_linear_kernel       one SM a tile of 8..128 channels x 16..256 tokens
+//   int8_linear_kernel       one SM a tile, either way
 //   int8_linear_pair_kernel  two SMs a tile of 256 x 256 (many tokens)
 // Every wait is bounded (mbar_wait_bounded); on a timeout all roles unwind.
 #pragma once
@@ -21,7 +23,7 @@
 
 namespace fmm {
 
-constexpr int kI8TileN = 128;    // output channels of an SM's tile
+constexpr int kI8Lanes = 128;    // MMA rows of an SM's tile
 constexpr int kI8BlockK = 128;   // k of one 128-byte swizzle row
 constexpr int kI8EpilogueWarps = 8;  // two for each 32 TMEM lanes, every other 32 columns each
 constexpr int kI8Threads = 64 + 32 * kI8EpilogueWarps;
@@ -34,10 +36,10 @@ struct Int8LinearParams {
   const float* channel_scales;
   const void* bias;  // output type, may be null
   void* out;
-  int32_t tok;       // tokens of a tile, a multiple of 16, <= 256
+  int32_t lanes;     // MMA rows of a tile: channels (a multiple of 8, <= 128), or 128 tokens
+  int32_t cols;      // MMA columns of a tile, a multiple of 16, <= 256: tokens, or channels
   int32_t stages;
-  int32_t rows;      // channels of a tile, a multiple of 8, <= 128
-  int32_t tiles_m, tiles_n;
+  int32_t tiles_m, tiles_n;  // token tiles, channel tiles
   int32_t group_m;   // token tiles of a group, which sweeps the channel tiles together
   int32_t atoms;     // 128-deep columns of a stage
   uint32_t tmem_cols;  // columns of one of the two accumulators
@@ -121,8 +123,7 @@ __device__ __forceinline__ float load_bias(const void* bias, int64_t n) {
 }
 
 // Scaled outputs of 32 token columns for one lane's channel: column c + j of
-// the tile is token m0 + c + j, lane j holds its scale.  A tile's columns are converted by one warp
-// each, so instructions count: whole blocks of 32 tokens x 32 channels take two
+// the tile is token m0 + c + j, lane j holds its scale.  Instructions count: whole blocks of 32 tokens x 32 channels take two
 // columns to a conversion and no predicates (9 instructions a column; 25 with a
 // branch a store, which held the 256 x 256 tiles back: 4096 x 4096 x 12288
 // 176 us).
@@ -151,11 +152,117 @@ __device__ __forceinline__ void store_columns(const Int8LinearParams& p, const u
   }
 }
 
+// Tiled TMA store (shared -> global) of one box; what lies outside is not written.
+__device__ __forceinline__ void tma_store_2d(const void* tmap, uint32_t src, int32_t c0, int32_t c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
+                   reinterpret_cast<uint64_t>(tmap)),
+               "r"(src), "r"(c0), "r"(c1)
+               : "memory");
+}
+
+// kTokens: 32 outputs of one lane's token, of channels n0 .. n0 + 31 (lane j
+// holds the scale and bias of channel n0 + j), into this lane's row of a 32 x
+// 32 block (64-byte swizzle: 16-byte unit j of row l sits at l * 64 + ((j ^ ((l
+// >> 1) & 3)) << 4)), which a TMA store writes.
+constexpr uint32_t kI8BlockBytes = 32 * 32 * 2;
+template <bool kBf16>
+__device__ __forceinline__ void store_block(const void* tmap, uint32_t buffer, const uint32_t (&v)[32], int64_t m,
+                                            int64_t n0, float token_scale, float channel_scale, float bias,
+                                            bool has_bias, int lane) {
+  uint32_t w[16];
+  if (has_bias) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2)
+      w[j / 2] = pack2_rn<kBf16>(
+          fmaf(static_cast<float>(static_cast<int32_t>(v[j])),
+               token_scale * __shfl_sync(0xffffffffu, channel_scale, j), __shfl_sync(0xffffffffu, bias, j)),
+          fmaf(static_cast<float>(static_cast<int32_t>(v[j + 1])),
+               token_scale * __shfl_sync(0xffffffffu, channel_scale, j + 1), __shfl_sync(0xffffffffu, bias, j + 1)));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2)
+      w[j / 2] = pack2_rn<kBf16>(static_cast<float>(static_cast<int32_t>(v[j])) *
+                                     (token_scale * __shfl_sync(0xffffffffu, channel_scale, j)),
+                                 static_cast<float>(static_cast<int32_t>(v[j + 1])) *
+                                     (token_scale * __shfl_sync(0xffffffffu, channel_scale, j + 1)));
+  }
+  // the store issued from this buffer two blocks ago must have read it
+  if (lane == 0) bulk_wait_group_read<1>();
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    st_shared_v4(buffer + static_cast<uint32_t>(lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)), w[4 * j], w[4 * j + 1],
+                 w[4 * j + 2], w[4 * j + 3]);
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) {
+    tma_store_2d(tmap, buffer, static_cast<int32_t>(n0), static_cast<int32_t>(m));
+    bulk_commit_group();
+  }
+}
+
+// One accumulator of 128 lanes x `columns` (of them `count` exist) at t_addr,
+// by one epilogue warp: its 32 lanes, every other 32 columns from `first` on.
+// lane0: what the warp's first lane stands for; column0: what column 0 does.
+template <bool kBf16, bool kTokens>
+struct Int8Epilogue {
+  const Int8LinearParams& p;
+  const void* tmap_c;
+  uint32_t buffers;  // kTokens: two blocks of this warp
+  int lane, first;
+  int turn = 0;
+
+  // scale and bias of lane's row, and the scale (and bias) of column first + lane
+  float row_scale, row_bias, col_scale, col_bias;
+  __device__ __forceinline__ void load_column(int64_t column0, int c, int count) {
+    const bool in = c + lane < count;
+    if constexpr (kTokens) {
+      col_scale = in ? p.channel_scales[column0 + c + lane] : 0.0f;
+      col_bias = in ? load_bias<kBf16>(p.bias, column0 + c + lane) : 0.0f;
+    } else {
+      col_scale = in ? p.token_scales[column0 + c + lane] : 0.0f;
+    }
+  }
+  __device__ __forceinline__ void prepare(int64_t row, int64_t column0, int count) {
+    if constexpr (kTokens) {
+      row_scale = row < p.M ? p.token_scales[row] : 0.0f;
+    } else {
+      row_scale = row < p.N ? p.channel_scales[row] : 0.0f;
+      row_bias = row < p.N ? load_bias<kBf16>(p.bias, row) : 0.0f;
+    }
+    load_column(column0, first, count);
+  }
+  __device__ __forceinline__ void drain(uint32_t t_addr, int64_t row, int64_t column0, int count) {
+#pragma unroll 1
+    for (int c = first; c < count; c += 64) {
+      uint32_t v[32];
+      tc_ld_32x32b_x32(t_addr + c, v);
+      const float scale = col_scale, bias = col_bias;
+      load_column(column0, c + 64, count);  // the next ones, before these are waited for
+      tc_wait_ld();
+      if constexpr (kTokens) {
+        if (row - lane < p.M)  // the warp's first token
+          store_block<kBf16>(tmap_c, buffers + (turn++ & 1) * kI8BlockBytes, v, row - lane, column0 + c, row_scale, scale,
+                             bias, p.bias != nullptr, lane);
+      } else {
+        store_columns<kBf16>(p, v, column0, c, count, row, scale, row_scale, row_bias);
+      }
+    }
+  }
+  __device__ __forceinline__ void finish() {
+    // the blocks must have been written before the CTA leaves
+    if constexpr (kTokens) {
+      if (lane == 0) bulk_wait_group_all();
+      __syncwarp();
+    }
+  }
+};
+
 // Structure (persistent over the tiles; 2 x tmem_cols accumulator columns, so
 // that the epilogue of a tile runs beside the next one's products):
-//   warp 0      TMA producer: a rows x 128 box of W and a tok x 128 box of Q a
-//               stage (128-byte swizzle; what lies outside reads as zero).
-//   warp 1      MMA issuer: 4 x m128 n<tok> k32 a stage; owns TMEM.
+//   warp 0      TMA producer: `atoms` lanes x 128 and cols x 128 boxes a stage
+//               (128-byte swizzle; what lies outside reads as zero).
+//   warp 1      MMA issuer: 4 x m128 n<cols> k32 a box; owns TMEM.
 //   warps 2..9  epilogue: tcgen05.ld 32 lanes x 32 columns, scale, bias, one
 //               rounding, 64-byte row segments.  Eight warps, because one to
 //               a scheduler waits for its own results (20000 x 256 x 1000:
@@ -164,19 +271,20 @@ __device__ __forceinline__ void store_columns(const Int8LinearParams& p, const u
 // cost the weight's bytes and little else, come out even over the SMs; the
 // product runs over 128 rows of shared memory all the same and the sums of the
 // rows behind the tile, whatever they are, are not read.
-template <bool kBf16>
+template <bool kBf16, bool kTokens>
 __global__ void __launch_bounds__(kI8Threads, 1)
-    int8_linear_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_q,
-                       const Int8LinearParams p) {
+    int8_linear_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                       const __grid_constant__ CUtensorMap tmap_c, const Int8LinearParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   const uint32_t base = (raw_addr + 1023u) & ~1023u;
-  const uint32_t tok_bytes = static_cast<uint32_t>(p.tok) * kI8BlockK;
-  const uint32_t w_bytes = static_cast<uint32_t>(p.rows) * kI8BlockK;
-  const uint32_t stage_bytes = p.atoms * (w_bytes + tok_bytes);
-  // tokens first: the products read 128 rows of W, into the next stage or, at
-  // the end, into what the host adds behind the last one
-  uint8_t* ctrl = smem_raw + (base - raw_addr) + p.stages * stage_bytes + (kI8TileN - p.rows) * kI8BlockK;
+  const uint32_t b_bytes = static_cast<uint32_t>(p.cols) * kI8BlockK;
+  const uint32_t a_bytes = static_cast<uint32_t>(p.lanes) * kI8BlockK;
+  const uint32_t stage_bytes = p.atoms * (a_bytes + b_bytes);
+  // columns first: the products read 128 rows of the other operand, into the
+  // next stage or, at the end, into what the host adds behind the last one
+  const uint32_t blocks = base + p.stages * stage_bytes + (kI8Lanes - p.lanes) * kI8BlockK;
+  uint8_t* ctrl = smem_raw + (blocks - raw_addr) + (kTokens ? kI8EpilogueWarps * 2 * kI8BlockBytes : 0);
   uint64_t* bars = reinterpret_cast<uint64_t*>(ctrl);
   const uint32_t full_bar = smem_u32(bars);
   const uint32_t empty_bar = smem_u32(bars + kI8MaxStages);
@@ -204,11 +312,11 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       const int atoms = min(p.atoms, columns - load_kb);
       const uint32_t bar = full_bar + 8 * load_stage;
       uint32_t dst = base + load_stage * stage_bytes;
-      mbar_arrive_expect_tx(bar, atoms * (w_bytes + tok_bytes));
+      mbar_arrive_expect_tx(bar, atoms * (a_bytes + b_bytes));
       for (int at = 0; at < atoms; ++at) {
-        tma_load_2d(dst + tok_bytes, &tmap_w, bar, (load_kb + at) * kI8BlockK, load_n * p.rows);
-        tma_load_2d(dst, &tmap_q, bar, (load_kb + at) * kI8BlockK, load_m * p.tok);
-        dst += w_bytes + tok_bytes;
+        tma_load_2d(dst + b_bytes, &tmap_a, bar, (load_kb + at) * kI8BlockK, (kTokens ? load_m : load_n) * p.lanes);
+        tma_load_2d(dst, &tmap_b, bar, (load_kb + at) * kI8BlockK, (kTokens ? load_n : load_m) * p.cols);
+        dst += a_bytes + b_bytes;
       }
     }
     __syncwarp();
@@ -236,8 +344,9 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     mbar_init(drain_bar, 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    prefetch_tmap(&tmap_w);
-    prefetch_tmap(&tmap_q);
+    prefetch_tmap(&tmap_a);
+    prefetch_tmap(&tmap_b);
+    if (kTokens) prefetch_tmap(&tmap_c);
   }
   if (warp == 0) {
     // the ring is filled while tensor memory is being allocated
@@ -270,9 +379,9 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     int stage = 0, acc = 0;
     uint32_t phase = 0, acc_phase = 0;
     bool ok = true, issued_any = false;
-    const uint32_t idesc = idesc_i8_s32(kI8TileN, static_cast<uint32_t>(p.tok));
-    const uint64_t q_desc0 = smem_desc_k_sw128(base), w_desc0 = smem_desc_k_sw128(base + tok_bytes);
-    const uint32_t atom_step = (w_bytes + tok_bytes) >> 4, stage_step = stage_bytes >> 4;
+    const uint32_t idesc = idesc_i8_s32(kI8Lanes, static_cast<uint32_t>(p.cols));
+    const uint64_t b_desc0 = smem_desc_k_sw128(base), a_desc0 = smem_desc_k_sw128(base + b_bytes);
+    const uint32_t atom_step = (a_bytes + b_bytes) >> 4, stage_step = stage_bytes >> 4;
     for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
       ok = __all_sync(0xffffffffu, mbar_wait_bounded(tempty_bar + 8 * acc, acc_phase ^ 1u, abort, p.timeout_ns, 22));
       if (!ok) break;
@@ -284,13 +393,13 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         tc_fence_after();
         if (elect_one()) {
           const int atoms = min(p.atoms, columns - kb);
-          uint64_t q_desc = q_desc0 + stage * stage_step, w_desc = w_desc0 + stage * stage_step;
+          uint64_t b_desc = b_desc0 + stage * stage_step, a_desc = a_desc0 + stage * stage_step;
           for (int at = 0; at < atoms; ++at) {
 #pragma unroll
             for (int kk = 0; kk < kI8BlockK / 32; ++kk)  // 32 codes on, 32 bytes on
-              tc_mma_i8(d_tmem, w_desc + kk * 2, q_desc + kk * 2, idesc, (kb > 0 || at > 0 || kk > 0) ? 1u : 0u);
-            q_desc += atom_step;
-            w_desc += atom_step;
+              tc_mma_i8(d_tmem, a_desc + kk * 2, b_desc + kk * 2, idesc, (kb > 0 || at > 0 || kk > 0) ? 1u : 0u);
+            b_desc += atom_step;
+            a_desc += atom_step;
           }
           tc_commit(empty_bar + 8 * stage);
         }
@@ -317,39 +426,27 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     }
   } else {
     const int quarter = warp & 3;  // TMEM lanes this warp may access
-    const int first = (warp - 2) / 4 * 32;
+    const int block = warp - 2;
+    Int8Epilogue<kBf16, kTokens> epilogue{p, &tmap_c, blocks + block * 2 * kI8BlockBytes, lane, block / 4 * 32};
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int t = blockIdx.x; t < total; t += gridDim.x) {
       int tm, tn;
       int8_tile_coords(p, t, tm, tn);
-      const int row = quarter * 32 + lane;
-      // a lane behind the tile has no channel
-      const int64_t n = row < p.rows ? static_cast<int64_t>(tn) * p.rows + row : p.N;
-      const int64_t m0 = static_cast<int64_t>(tm) * p.tok;
-      const int tokens = static_cast<int>(p.M - m0 < p.tok ? p.M - m0 : p.tok);
-      const float channel_scale = n < p.N ? p.channel_scales[n] : 0.0f;
-      const float bias = n < p.N ? load_bias<kBf16>(p.bias, n) : 0.0f;
-      float token_scale = first + lane < tokens ? p.token_scales[m0 + first + lane] : 0.0f;
+      // lanes behind the tile or the operand stand for its end
+      const int64_t lane_end = kTokens ? p.M : p.N, lane0 = static_cast<int64_t>(kTokens ? tm : tn) * p.lanes;
+      const int64_t row = quarter * 32 + lane < p.lanes ? lane0 + quarter * 32 + lane : lane_end;
+      const int64_t column0 = static_cast<int64_t>(kTokens ? tn : tm) * p.cols;
+      const int64_t rest = (kTokens ? p.N : p.M) - column0;
+      const int count = static_cast<int>(rest < p.cols ? rest : p.cols);
+      epilogue.prepare(row, column0, count);
       int ready = 0;
       if (lane == 0) ready = mbar_wait_bounded(tfull_bar + 8 * acc, acc_phase, abort, p.timeout_ns, 24) ? 1 : 0;
       ready = __shfl_sync(0xffffffffu, ready, 0);
       if (!ready) break;
       tc_fence_after();
-      const uint32_t t_addr = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * p.tmem_cols;
-      if (quarter * 32 < p.rows) {
-#pragma unroll 1
-        for (int c = first; c < tokens; c += 64) {
-          uint32_t v[32];
-          tc_ld_32x32b_x32(t_addr + c, v);
-          // the next columns' scales, before they are waited for
-          const int next = c + 64 + lane;
-          const float next_scale = next < tokens ? p.token_scales[m0 + next] : 0.0f;
-          tc_wait_ld();
-          store_columns<kBf16>(p, v, m0, c, tokens, n, token_scale, channel_scale, bias);
-          token_scale = next_scale;
-        }
-      }
+      if (quarter * 32 < p.lanes)
+        epilogue.drain(tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * p.tmem_cols, row, column0, count);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(tempty_bar + 8 * acc);
@@ -358,6 +455,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         acc_phase ^= 1u;
       }
     }
+    epilogue.finish();
   }
 
   tc_fence_before();
@@ -370,8 +468,8 @@ __global__ void __launch_bounds__(kI8Threads, 1)
 
 // ---------------------------------------------------------------------------
 // 2-SM form: a cluster of two CTAs computes a tile of 256 channels x 256 tokens
-// with tcgen05.mma.cta_group::2.  CTA r holds channels [128 r, 128 r + 128) of
-// the W tile and its half of the tokens, so an SM loads 32 KB a 128-deep block
+// with tcgen05.mma.cta_group::2.  CTA r holds channels [128 r, 128 r + 128) and
+// its half of the tokens, so an SM loads 32 KB a 128-deep block
 // for twice the products that the same bytes give one SM alone: at the full
 // rate L2 and shared memory are what bounds the product, not the tensor cores.
 // Roles as above; the even CTA issues the products, loads complete on its
@@ -381,7 +479,7 @@ struct Int8PairConfig {
   static constexpr int kAtoms = 2;  // 128-deep columns of swizzle atoms a stage
   static constexpr int kBK = kAtoms * kI8BlockK;
   static constexpr int kStages = 3;
-  static constexpr uint32_t kAtomBytes = 128 * kI8BlockK;      // this CTA's half of W or Q
+  static constexpr uint32_t kAtomBytes = 128 * kI8BlockK;      // this CTA's half of an operand
   static constexpr uint32_t kABytes = kAtoms * kAtomBytes;     // 32 KB
   static constexpr uint32_t kStageBytes = 2 * kABytes;         // 64 KB
   static constexpr size_t kSmemBytes = size_t(kStages) * kStageBytes + 1024 + 8 * (2 * kStages + 8);
@@ -389,8 +487,8 @@ struct Int8PairConfig {
 
 template <bool kBf16>
 __global__ void __launch_bounds__(kI8Threads, 1)
-    int8_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_q,
-                            const __grid_constant__ CUtensorMap tmap_q16, const Int8LinearParams p) {
+    int8_linear_pair_kernel(const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_b,
+                            const __grid_constant__ CUtensorMap tmap_b16, const Int8LinearParams p) {
   using Cfg = Int8PairConfig;
   constexpr int STAGES = Cfg::kStages;
   extern __shared__ uint8_t smem_raw[];
@@ -421,9 +519,9 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     mbar_init(drain_bar, 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    prefetch_tmap(&tmap_w);
-    prefetch_tmap(&tmap_q);
-    prefetch_tmap(&tmap_q16);
+    prefetch_tmap(&tmap_a);
+    prefetch_tmap(&tmap_b);
+    prefetch_tmap(&tmap_b16);
   }
   if (warp == 1) {
     tmem_alloc_pair(smem_u32(tmem_slot), 2 * Cfg::kTile);
@@ -436,7 +534,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
 
   const int total = p.tiles_m * p.tiles_n;
   const int k_blocks = static_cast<int>((p.K + Cfg::kBK - 1) / Cfg::kBK);
-  // token columns of tile tm: the MMA's N, 16 from each CTA at least
+  // columns of tile tm: the MMA's N, 16 from each CTA at least
   auto columns = [&](int tm) {
     const int64_t rest = p.M - static_cast<int64_t>(tm) * Cfg::kTile;
     return rest >= Cfg::kTile ? Cfg::kTile : static_cast<int>((rest + 31) / 32 * 32);
@@ -453,8 +551,8 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       // exactly its half in 16-row boxes, since a 128-row box would fetch
       // rows that belong to the other half
       const int n_cols = columns(tm), half = n_cols / 2;
-      const int w_row = tn * Cfg::kTile + static_cast<int>(cta) * 128;
-      const int q_row = tm * Cfg::kTile + static_cast<int>(cta) * half;
+      const int a_row = tn * Cfg::kTile + static_cast<int>(cta) * 128;
+      const int b_row = tm * Cfg::kTile + static_cast<int>(cta) * half;
       const uint32_t stage_tx = 2u * (Cfg::kABytes + static_cast<uint32_t>(half) * Cfg::kBK);
       for (int kb = 0; kb < k_blocks; ++kb) {
         ok = __all_sync(0xffffffffu,
@@ -466,14 +564,14 @@ __global__ void __launch_bounds__(kI8Threads, 1)
 #pragma unroll
           for (int at = 0; at < Cfg::kAtoms; ++at) {
             const int k0 = kb * Cfg::kBK + at * kI8BlockK;
-            const uint32_t w_dst = base + stage * Cfg::kStageBytes + at * Cfg::kAtomBytes;
-            const uint32_t q_dst = w_dst + Cfg::kABytes;
-            tma_load_2d_pair(w_dst, &tmap_w, full_even, k0, w_row);
+            const uint32_t a_dst = base + stage * Cfg::kStageBytes + at * Cfg::kAtomBytes;
+            const uint32_t b_dst = a_dst + Cfg::kABytes;
+            tma_load_2d_pair(a_dst, &tmap_a, full_even, k0, a_row);
             if (n_cols == Cfg::kTile) {
-              tma_load_2d_pair(q_dst, &tmap_q, full_even, k0, q_row);
+              tma_load_2d_pair(b_dst, &tmap_b, full_even, k0, b_row);
             } else {
               for (int j = 0; j < half; j += 16)
-                tma_load_2d_pair(q_dst + static_cast<uint32_t>(j) * kI8BlockK, &tmap_q16, full_even, k0, q_row + j);
+                tma_load_2d_pair(b_dst + static_cast<uint32_t>(j) * kI8BlockK, &tmap_b16, full_even, k0, b_row + j);
             }
           }
         }
@@ -497,7 +595,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true, issued_any = false;
-      const uint64_t w_desc0 = smem_desc_k_sw128(base), q_desc0 = smem_desc_k_sw128(base + Cfg::kABytes);
+      const uint64_t a_desc0 = smem_desc_k_sw128(base), b_desc0 = smem_desc_k_sw128(base + Cfg::kABytes);
       for (int t = pair; t < total && ok; t += pairs) {
         int tm, tn;
         int8_tile_coords(p, t, tm, tn);
@@ -513,12 +611,12 @@ __global__ void __launch_bounds__(kI8Threads, 1)
           if (!ok) break;
           tc_fence_after();
           if (elect_one()) {
-            const uint64_t w_desc = w_desc0 + stage * (Cfg::kStageBytes >> 4);
-            const uint64_t q_desc = q_desc0 + stage * (Cfg::kStageBytes >> 4);
+            const uint64_t a_desc = a_desc0 + stage * (Cfg::kStageBytes >> 4);
+            const uint64_t b_desc = b_desc0 + stage * (Cfg::kStageBytes >> 4);
 #pragma unroll
             for (int kk = 0; kk < Cfg::kBK / 32; ++kk) {
               const uint32_t at = (kk / 4) * (Cfg::kAtomBytes >> 4) + (kk % 4) * 2;
-              tc_mma_i8_pair(d_tmem, w_desc + at, q_desc + at, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+              tc_mma_i8_pair(d_tmem, a_desc + at, b_desc + at, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
             }
             tc_commit_pair_multicast(empty_bar + 8 * stage, 0x3);
           }
@@ -546,37 +644,26 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     }
   } else {
     const int quarter = warp & 3;
-    const int first = (warp - 2) / 4 * 32;
     const uint32_t tempty_even = map_to_cta(tempty_bar, 0);
+    Int8Epilogue<kBf16, false> epilogue{p, nullptr, 0u, lane, (warp - 2) / 4 * 32};
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int t = pair; t < total; t += pairs) {
       int tm, tn;
       int8_tile_coords(p, t, tm, tn);
-      const int64_t n = static_cast<int64_t>(tn) * Cfg::kTile + static_cast<int>(cta) * 128 + quarter * 32 + lane;
-      const int64_t m0 = static_cast<int64_t>(tm) * Cfg::kTile;
-      const int tokens = static_cast<int>(p.M - m0 < Cfg::kTile ? p.M - m0 : Cfg::kTile);
-      const float channel_scale = n < p.N ? p.channel_scales[n] : 0.0f;
-      const float bias = n < p.N ? load_bias<kBf16>(p.bias, n) : 0.0f;
-      float token_scale = first + lane < tokens ? p.token_scales[m0 + first + lane] : 0.0f;
+      const int64_t row = static_cast<int64_t>(tn) * Cfg::kTile + static_cast<int>(cta) * 128 + quarter * 32 + lane;
+      const int64_t column0 = static_cast<int64_t>(tm) * Cfg::kTile;
+      const int count = static_cast<int>(p.M - column0 < Cfg::kTile ? p.M - column0 : Cfg::kTile);
+      epilogue.prepare(row, column0, count);
       int ready = 0;
       if (lane == 0)
         ready = mbar_wait_bounded_cluster(tfull_bar + 8 * acc, acc_phase, abort, p.timeout_ns, 44) ? 1 : 0;
       ready = __shfl_sync(0xffffffffu, ready, 0);
       if (!ready) break;
       tc_fence_after();
-      const uint32_t t_addr =
-          tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * Cfg::kTile);
-#pragma unroll 1
-      for (int c = first; c < tokens; c += 64) {
-        uint32_t v[32];
-        tc_ld_32x32b_x32(t_addr + c, v);
-        const int next = c + 64 + lane;
-        const float next_scale = next < tokens ? p.token_scales[m0 + next] : 0.0f;
-        tc_wait_ld();
-        store_columns<kBf16>(p, v, m0, c, tokens, n, token_scale, channel_scale, bias);
-        token_scale = next_scale;
-      }
+      epilogue.drain(
+          tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + static_cast<uint32_t>(acc * Cfg::kTile), row, column0,
+          count);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_remote(tempty_even + 8 * acc);

@@ -287,7 +287,9 @@ SHAPES = [(1, 1, 1), (1, 128, 128), (2, 17, 31), (7, 129, 300), (15, 16, 129), (
           # 128 channels, pairs of SMs with whole and ragged token tiles
           (1, 1040, 500), (2, 2063, 4001), (4, 1025, 3600), (4, 4096, 131), (1, 4609, 8001), (2, 1024, 7300),
           (5, 300, 9000), (48, 1100, 8200), (200, 2000, 4100), (700, 515, 9001), (600, 4096, 9472),
-          (1300, 1031, 4999), (300, 1024, 37889)]
+          (1300, 1031, 4999), (300, 1024, 37889),
+          # a short K with many outputs: tokens in the lanes where rows of 8 outputs are aligned
+          (3000, 64, 1000), (20003, 100, 304), (2500, 33, 72), (5000, 257, 520), (9000, 16, 8), (4001, 128, 1001)]
 
 
 @pytest.mark.parametrize("with_bias", [False, True])
