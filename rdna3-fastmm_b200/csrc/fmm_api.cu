@@ -1044,7 +1044,8 @@ bool plan_streamed_rows(Int8RowsParams* p, size_t slot, size_t code_bytes, size_
   if (warps > ceil_div(vectors, 32)) warps = ceil_div(vectors, 32);
   if (warps < 1) warps = 1;
   if (warps > 1 && groups > 15) groups = 15;
-  if (groups * warps > 32) groups = 32 / warps;
+  const int64_t total = (code_bytes == 0 && gain_bytes > 0 ? kRowsNormThreads : kRowsMaxThreads) / 32;
+  if (groups * warps > total) groups = total / warps;
   p->groups = static_cast<int32_t>(groups);
   p->warps_per_row = static_cast<int32_t>(warps);
   p->stages = kRowsMaxStages;

@@ -33,6 +33,7 @@
 namespace fmm {
 
 constexpr int kRowsMaxThreads = 1024;
+constexpr int kRowsNormThreads = 768;  // streamed norms: 80 registers a thread (65536 x 4608: 349 us with 64, 333)
 
 struct Int8RowsParams {
   const void* x;
@@ -456,7 +457,7 @@ constexpr int kRowsMaxStages = 4;
 // into the stage by threads; accesses are one element wide, `width` threads
 // apart, and codes are collected in shared memory.
 template <class T, class G, bool kNorm, bool kVec>
-__global__ void __launch_bounds__(kRowsMaxThreads, 1) int8_rows_streamed_kernel(const Int8RowsParams p) {
+__global__ void __launch_bounds__(kVec && kNorm ? kRowsNormThreads : kRowsMaxThreads, 1) int8_rows_streamed_kernel(const Int8RowsParams p) {
   constexpr bool kPair = kNorm && std::is_same<G, float>::value;
   __shared__ __align__(8) uint64_t s_full[kRowsMaxGroups * kRowsMaxStages];
   __shared__ float s_square[kRowsMaxGroups];
