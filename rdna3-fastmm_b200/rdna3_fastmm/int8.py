@@ -46,6 +46,7 @@ __all__ = [
 ]
 
 CODE_ALIGNMENT = 16
+_INF = float("inf")
 MAX_INNER = 131071  # 2^14 a product of two codes of -128, sums below 2^31
 _HALF_TYPES = (torch.bfloat16, torch.float16)
 
@@ -72,6 +73,10 @@ def empty_codes(shape: tuple[int, ...], device: torch.device) -> torch.Tensor:
 # ---------------------------------------------------------------- operands
 # A call between two single tokens is a few microseconds of GPU time, so the
 # checks below read each tensor's attributes once and pass plain integers on.
+_BF16, _FP16, _FP32, _INT8 = torch.bfloat16, torch.float16, torch.float32, torch.int8
+_grad_enabled = torch.is_grad_enabled
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
 _ROW_TYPES = {torch.bfloat16: _native.FMM_DTYPE_BF16, torch.float16: _native.FMM_DTYPE_F16,
               torch.float32: _native.FMM_DTYPE_F32}
 
@@ -86,7 +91,7 @@ def _flat(tensor: torch.Tensor) -> tuple[int, int, int] | None:
     shape = tensor.shape
     inner = shape[-1]
     if inner and tensor.is_contiguous():
-        rows = tensor.numel() // inner
+        rows = shape[0] if len(shape) == 2 else tensor.numel() // inner
         # a single row has no second one to reach
         return rows, inner, inner if rows > 1 else (inner + 15) & -16
     rows, pitch, step = 1, None, None
@@ -123,12 +128,13 @@ def _output_rows(tensor: torch.Tensor, shape: torch.Size, dtype: torch.dtype, de
         raise ValueError(f"{name} has shape {tuple(tensor.shape)}, expected {tuple(shape)}")
     if tensor.get_device() != device or tensor.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype} on cuda:{device}")
-    if like is not None and (rows := _like(tensor, like)) is not None:
-        return rows
+    if like is not None and tensor.is_contiguous():
+        _, rows, inner, _, _ = like
+        return tensor.data_ptr(), rows, inner, inner if rows > 1 else (inner + 15) & -16, dtype.itemsize
     flat = _flat(tensor)
     if flat is None:
         raise ValueError(f"{name} must have dense rows a constant step apart")
-    return tensor.data_ptr(), *flat, tensor.element_size()
+    return tensor.data_ptr(), *flat, dtype.itemsize
 
 
 def _like(tensor: torch.Tensor, rows: _Rows) -> _Rows | None:
@@ -142,7 +148,7 @@ def _like(tensor: torch.Tensor, rows: _Rows) -> _Rows | None:
 def _input_scales(tensor: torch.Tensor, shape: torch.Size, device: int, name: str) -> torch.Tensor:
     if tensor.shape != shape:
         raise ValueError(f"{name} has shape {tuple(tensor.shape)}, expected {tuple(shape)}")
-    if tensor.get_device() != device or tensor.dtype is not torch.float32:
+    if tensor.get_device() != device or tensor.dtype is not _FP32:
         raise ValueError(f"{name} must be float32 on cuda:{device}")
     return tensor if tensor.is_contiguous() else tensor.contiguous()
 
@@ -150,15 +156,15 @@ def _input_scales(tensor: torch.Tensor, shape: torch.Size, device: int, name: st
 def _output_scales(tensor: torch.Tensor, shape: torch.Size, device: int) -> None:
     if tensor.shape != shape:
         raise ValueError(f"scales has shape {tuple(tensor.shape)}, expected {tuple(shape)}")
-    if tensor.get_device() != device or tensor.dtype is not torch.float32 or not tensor.is_contiguous():
+    if tensor.get_device() != device or tensor.dtype is not _FP32 or not tensor.is_contiguous():
         raise ValueError(f"scales must be contiguous float32 on cuda:{device}")
 
 
 def _refuse_grad(*tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled():
-        for tensor in tensors:
-            if tensor is not None and tensor.requires_grad:
-                raise ValueError("the B200 8-bit operators do not support autograd")
+    """Called while gradients are enabled."""
+    for tensor in tensors:
+        if tensor is not None and tensor.requires_grad:
+            raise ValueError("the B200 8-bit operators do not support autograd")
 
 
 def _require_cuda(tensor: torch.Tensor, name: str) -> int:
@@ -215,14 +221,21 @@ def _refuse_overlap(outputs: list[_Rows], inputs: list[_Rows]) -> None:
                 raise ValueError("output storage must not overlap inputs or other outputs")
 
 
+_entry_points: dict = {}
+
+
+def _entry_point(name: str):
+    return _entry_points.setdefault(name, _native.entry_point(name))
+
+
 def _launch(device: int, name: str, *args) -> None:
     """Call the C entry point with ``device`` current, on its current stream."""
-    function = _native.entry_point(name)
-    if device == torch._C._cuda_getDevice():
-        code = function(*args, torch._C._cuda_getCurrentRawStream(device))
+    function = _entry_points.get(name) or _entry_point(name)
+    if device == _current_device():
+        code = function(*args, _current_stream(device))
     else:
         with torch.cuda.device(device):
-            code = function(*args, torch._C._cuda_getCurrentRawStream(device))
+            code = function(*args, _current_stream(device))
     if code:
         _native.check(code, name)
 
@@ -243,14 +256,15 @@ def quantize_rows(x: torch.Tensor, *, codes: torch.Tensor | None = None,
     shape = x.shape
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError("x must have a last dimension of at least one element")
-    _refuse_grad(x, codes, scales)
+    if _grad_enabled():
+        _refuse_grad(x, codes, scales)
     held, source = _input_rows(x)
     leading = shape[:-1]
     if codes is None:
         codes = empty_codes(shape, x.device)
     if scales is None:
         scales = torch.empty(leading, device=x.device, dtype=torch.float32)
-    q = _output_rows(codes, shape, torch.int8, device, "codes", source)
+    q = _output_rows(codes, shape, _INT8, device, "codes", source)
     _output_scales(scales, leading, device)
     rows = source[1]
     s = scales.data_ptr(), 1 if rows else 0, rows, rows, 4
@@ -272,7 +286,7 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
     updates the stream in place."""
     device = _require_cuda(x, "x")
     kind = x.dtype
-    if kind not in _HALF_TYPES:
+    if kind is not _BF16 and kind is not _FP16:
         raise ValueError(f"rms_norm_int8 takes BF16 or FP16 rows, not {kind}")
     shape = x.shape
     if len(shape) < 1 or shape[-1] < 1:
@@ -280,24 +294,25 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
     if weight.shape != shape[-1:]:
         raise ValueError(f"weight has shape {tuple(weight.shape)}, expected {tuple(shape[-1:])}")
     gain_kind = weight.dtype
-    if weight.get_device() != device or (gain_kind is not kind and gain_kind is not torch.float32):
+    if weight.get_device() != device or (gain_kind is not kind and gain_kind is not _FP32):
         raise ValueError("weight must have x's dtype or float32, on x's device")
-    if not 0.0 <= eps < float("inf"):
+    if not 0.0 <= eps < _INF:
         raise ValueError("eps must be finite and not negative")
     if residual is None and residual_out is not None:
         raise ValueError("residual_out needs a residual")
-    _refuse_grad(x, weight, residual, codes, scales, residual_out)
+    if _grad_enabled():
+        _refuse_grad(x, weight, residual, codes, scales, residual_out)
     held, source = _input_rows(x)
     if not weight.is_contiguous():
         weight = weight.contiguous()
     ptr, rows, inner, pitch, _ = source
-    gain = weight.data_ptr(), 1, inner, inner, 4 if gain_kind is torch.float32 else 2
+    gain = weight.data_ptr(), 1, inner, inner, 4 if gain_kind is _FP32 else 2
     leading = shape[:-1]
     if codes is None:
         codes = empty_codes(shape, x.device)
     if scales is None:
         scales = torch.empty(leading, device=x.device, dtype=torch.float32)
-    q = _output_rows(codes, shape, torch.int8, device, "codes", source)
+    q = _output_rows(codes, shape, _INT8, device, "codes", source)
     _output_scales(scales, leading, device)
     s = scales.data_ptr(), 1 if rows else 0, rows, rows, 4
     if residual is None:
@@ -338,7 +353,7 @@ def linear_int8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.T
     and rounded once.  Code rows must start on 16-byte boundaries, as
     ``quantize_rows``, ``rms_norm_int8`` and ``empty_codes`` make them."""
     device = _require_cuda(codes, "codes")
-    if (codes.dtype is not torch.int8 or weight_codes.dtype is not torch.int8
+    if (codes.dtype is not _INT8 or weight_codes.dtype is not _INT8
             or weight_codes.get_device() != device):
         raise ValueError("codes and weight_codes must be int8 tensors of one device")
     token_shape, weight_shape = codes.shape, weight_codes.shape
@@ -351,9 +366,10 @@ def linear_int8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.T
         raise ValueError(f"K = {inner} could leave the 32-bit sum (at most {MAX_INNER})")
     if dtype is None:
         dtype = out.dtype if out is not None else bias.dtype if bias is not None else torch.bfloat16
-    if dtype not in _HALF_TYPES:
+    if dtype is not _BF16 and dtype is not _FP16:
         raise ValueError(f"linear_int8 writes BF16 or FP16, not {dtype}")
-    _refuse_grad(scales, weight_scales, bias, out)
+    if _grad_enabled():
+        _refuse_grad(scales, weight_scales, bias, out)
     q, w = _flat(codes), _flat(weight_codes)
     if q is None or w is None:
         raise ValueError("codes must have dense rows a constant step apart")
