@@ -162,7 +162,8 @@ __device__ __forceinline__ RowScale row_scale(const RowTotals& total) {
 template <bool kNorm>
 __device__ __forceinline__ float stored_scale(const RowTotals& total, const RowScale& s, int cols, float eps) {
   float scale = __uint_as_float(total.peak);
-  if constexpr (kNorm) scale = scale / sqrtf(total.square / static_cast<float>(cols) + eps);
+  // a row of zeros has scale 0, without an epsilon too
+  if (kNorm && total.peak != 0u) scale = scale / sqrtf(total.square / static_cast<float>(cols) + eps);
   return s.finite ? scale / 127.0f : __uint_as_float(0x7fc00000u);
 }
 
@@ -457,7 +458,8 @@ constexpr int kRowsMaxStages = 4;
 // into the stage by threads; accesses are one element wide, `width` threads
 // apart, and codes are collected in shared memory.
 template <class T, class G, bool kNorm, bool kVec>
-__global__ void __launch_bounds__(kVec && kNorm ? kRowsNormThreads : kRowsMaxThreads, 1) int8_rows_streamed_kernel(const Int8RowsParams p) {
+__global__ void __launch_bounds__(kVec && kNorm ? kRowsNormThreads : kRowsMaxThreads, 1)
+    int8_rows_streamed_kernel(const Int8RowsParams p) {
   constexpr bool kPair = kNorm && std::is_same<G, float>::value;
   __shared__ __align__(8) uint64_t s_full[kRowsMaxGroups * kRowsMaxStages];
   __shared__ float s_square[kRowsMaxGroups];

@@ -477,8 +477,8 @@ class Int8Plan:
         self._validate_input(input_tensor)
         self._validate_packed(weight)
         self._validate_workspace(workspace)
+        self._validate_product(workspace, weight, bias, output)
         self._refuse_output(output, input_tensor)
-        self._refuse_weight(workspace, weight)
         quantize_rows(input_tensor, codes=workspace.codes, scales=workspace.scales)
         return linear_int8(workspace.codes, workspace.scales, weight.codes, weight.scales, bias, dtype=self.dtype,
                            out=output)
@@ -493,9 +493,9 @@ class Int8Plan:
         self._validate_input(input_tensor)
         self._validate_packed(weight)
         self._validate_workspace(workspace)
+        self._validate_product(workspace, weight, bias, output)
         self._refuse_output(output, input_tensor, norm_weight, residual, residual_output)
         self._refuse_output(residual_output, weight.codes, weight.scales, bias)
-        self._refuse_weight(workspace, weight)
         stream = rms_norm_int8(input_tensor, norm_weight, residual, eps, codes=workspace.codes,
                                scales=workspace.scales, residual_out=residual_output).residual
         result = linear_int8(workspace.codes, workspace.scales, weight.codes, weight.scales, bias, dtype=self.dtype,
@@ -522,12 +522,28 @@ class Int8Plan:
                 or tuple(workspace.codes.shape) != (self.rows, self.inner)):
             raise ValueError("workspace does not match the plan")
 
-    @staticmethod
-    def _refuse_weight(workspace: Int8Workspace, weight: Int8PackedWeight) -> None:
-        for buffer in (workspace.codes, workspace.scales):
-            for packed in (weight.codes, weight.scales):
-                if _rows_overlap(_input_rows(buffer)[1], _input_rows(packed)[1]):
-                    raise ValueError("work buffers must not overlap")
+    def _validate_product(self, workspace: Int8Workspace, weight: Int8PackedWeight, bias: torch.Tensor | None,
+                          output: torch.Tensor | None) -> None:
+        """What the product would refuse, before the first kernel has changed anything."""
+        buffers = [_input_rows(buffer)[1] for buffer in (workspace.codes, workspace.scales)]
+        packed = [_input_rows(tensor)[1] for tensor in (weight.codes, weight.scales)]
+        if any(_rows_overlap(buffer, tensor) for buffer in buffers for tensor in packed):
+            raise ValueError("work buffers must not overlap")
+        if bias is not None:
+            if tuple(bias.shape) != (self.columns,):
+                raise ValueError(f"bias matrix has shape {tuple(bias.shape)}, expected {(self.columns,)}")
+            if bias.device != self.device or bias.dtype != self.dtype:
+                raise ValueError("bias matrix device or dtype does not match the plan")
+            if _grad_enabled():
+                _refuse_grad(bias)
+        if output is not None:
+            rows = _output_rows(output, torch.Size((self.rows, self.columns)), self.dtype, self.device.index, "output")
+            if _grad_enabled():
+                _refuse_grad(output)
+            if bias is not None:
+                packed.append(_input_rows(bias)[1])
+            if any(_rows_overlap(rows, tensor) for tensor in buffers + packed):
+                raise ValueError("output storage must not overlap inputs or workspace")
 
     @staticmethod
     def _refuse_output(output: torch.Tensor | None, *tensors: torch.Tensor | None) -> None:

@@ -158,6 +158,38 @@ def test_many_rows_stream_through(rows, inner, gain, with_residual):
     assert bool(((scales.double() - peak / 127.0).abs() <= U32 * peak / 127.0).all())
 
 
+@pytest.mark.parametrize("rows", [2, 5000])
+def test_zeros_without_an_epsilon(rows):
+    x = torch.zeros((rows, 1024), dtype=BF16, device=DEVICE)
+    x[1] = 1
+    codes, scales, _ = rms_norm_int8(x, torch.ones(1024, device=DEVICE), eps=0.0)
+    assert not codes[0].any() and scales[0] == 0 and bool((codes[1] == 127).all())
+    assert bool((scales[2:] == 0).all()) and abs(scales[1].item() - 1 / 127) <= 4 * U32
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^32 bytes and 2^31 elements; the last rows come out as alone."""
+    rows, inner = 70000, 32768
+    x = torch.zeros((rows, inner), dtype=BF16, device=DEVICE)
+    x[-3:] = _randn((3, inner), 1, BF16).to(DEVICE)
+    codes, scales = quantize_rows(x)
+    alone = quantize_rows(x[-3:].clone())
+    assert torch.equal(codes[-3:], alone.codes) and torch.equal(scales[-3:], alone.scales)
+    weight = torch.ones(inner, device=DEVICE)
+    got = rms_norm_int8(x, weight, x, codes=codes, scales=scales, residual_out=x)
+    again = rms_norm_int8(got.residual[-3:].clone() / 2, weight, got.residual[-3:].clone() / 2)
+    assert torch.equal(got.codes[-3:], again.codes) and torch.equal(got.residual[-3:], again.residual)
+    del x, got
+    w, ws = quantize_rows(_randn((40, inner), 2).to(DEVICE))
+    y = linear_int8(codes, scales, w, ws)
+    assert torch.equal(y[-3:], linear_int8(codes[-3:], scales[-3:], w, ws))
+    del codes, y
+    q, s = quantize_rows(_randn((300000, 64), 3).to(DEVICE))
+    w, ws = quantize_rows(_randn((8200, 64), 4).to(DEVICE))
+    y = linear_int8(q, s, w, ws)
+    assert torch.equal(y[-5:], linear_int8(q[-5:], s[-5:], w, ws))
+
+
 @pytest.mark.parametrize("scale", [2.0**-130, 2.0**-110, 2.0**100])
 def test_rows_of_extreme_magnitude(scale):
     x = (_randn((3, 700), 5).to(BF16).double() * scale).to(FP32)
@@ -565,6 +597,15 @@ def test_plan_refusals():
     with pytest.raises(ValueError, match="overlap"):
         plan.run_norm_linear_packed(x, torch.ones(64, device=DEVICE), packed, ws, r, output=r[:, :8],
                                     residual_output=r)
+    # a product that is refused leaves the stream as it was
+    before = r.clone()
+    for wrong in (dict(bias=torch.ones(8, device=DEVICE)), dict(bias=torch.ones(9, dtype=BF16, device=DEVICE)),
+                  dict(output=torch.empty((4, 9), dtype=BF16, device=DEVICE)),
+                  dict(output=torch.empty((4, 8), dtype=FP16, device=DEVICE)),
+                  dict(output=ws.codes.view(BF16)[:, :8])):
+        with pytest.raises(ValueError):
+            plan.run_norm_linear_packed(x, torch.ones(64, device=DEVICE), packed, ws, r, residual_output=r, **wrong)
+    assert torch.equal(r, before)
     other = Int8Plan(6, 64, 8, DEVICE)
     out = other.run_linear_packed(torch.ones((6, 64), dtype=BF16, device=DEVICE), packed,
                                   other.allocate_workspace(0.1))
