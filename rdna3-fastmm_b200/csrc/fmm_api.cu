@@ -1002,6 +1002,30 @@ int launch_leaf_gemm(int rank, const void* L, const void* Rt, int64_t bm, int64_
 }
 
 // ------------------------------------------------------------------ 8-bit integer linear
+// Launch that may overlap the end of the kernel before it in the stream
+// (wait_for_previous_kernel), in clusters of `cluster` CTAs.
+template <class... P, class... A>
+int launch_int8(void (*kernel)(P...), const char* what, int64_t grid, int threads, size_t shared, int cluster,
+                cudaStream_t stream, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads), 1, 1);
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) return cuda_fail(e, what);
+  return FMM_OK;
+}
+
 template <class T, class G, bool kNorm, int V, bool kVec>
 int launch_int8_rows(const Int8RowsParams& p, int threads, const DeviceInfo* info, cudaStream_t stream) {
   const int rows_per_block = p.warps_per_row > 1 ? 1 : threads / 32;
@@ -1009,10 +1033,8 @@ int launch_int8_rows(const Int8RowsParams& p, int threads, const DeviceInfo* inf
   // the blocks that an SM is sure to hold at once (64 registers a thread); each takes row after row
   const int64_t cap = int64_t(usable_sms(info)) * (kRowsMaxThreads / threads);
   const int grid = static_cast<int>(blocks < cap ? blocks : cap);
-  int8_rows_kernel<T, G, kNorm, V, kVec><<<grid, threads, 0, stream>>>(p);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, kNorm ? "RMS norm (8-bit) launch" : "row quantisation launch");
-  return FMM_OK;
+  return launch_int8(int8_rows_kernel<T, G, kNorm, V, kVec>,
+                     kNorm ? "RMS norm (8-bit) launch" : "row quantisation launch", grid, threads, 0, 1, stream, p);
 }
 
 constexpr size_t kRowsRingBytes = 216 * 1024;  // rings of the streamed form
@@ -1068,10 +1090,8 @@ int launch_int8_rows_streamed(Int8RowsParams p, size_t shared, const DeviceInfo*
   const int64_t blocks = ceil_div(p.rows, p.groups);
   const int sms = usable_sms(info);
   const int grid = static_cast<int>(blocks < sms ? blocks : sms);
-  kernel<<<grid, 32 * p.warps_per_row * p.groups, shared, stream>>>(p);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, kNorm ? "RMS norm (8-bit) launch" : "row quantisation launch");
-  return FMM_OK;
+  return launch_int8(kernel, kNorm ? "RMS norm (8-bit) launch" : "row quantisation launch", grid,
+                     32 * p.warps_per_row * p.groups, shared, 1, stream, p);
 }
 
 // Many rows are streamed.  Otherwise a row of up to 1024 elements is one
@@ -1271,10 +1291,8 @@ int launch_int8_single(const int8_t* codes, int64_t ldq, const int8_t* weight_co
   }
   const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n;
   const int grid = static_cast<int>(tiles < sms ? tiles : sms);
-  int8_linear_kernel<kBf16, kTokens><<<grid, kI8Threads, smem, stream>>>(map_a, map_b, map_c, p);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "8-bit linear launch");
-  return FMM_OK;
+  return launch_int8(int8_linear_kernel<kBf16, kTokens>, "8-bit linear launch", grid, kI8Threads, smem, 1, stream,
+                     map_a, map_b, map_c, p);
 }
 
 template <bool kBf16>
@@ -1297,21 +1315,8 @@ int launch_int8_pair(const int8_t* codes, int64_t ldq, const int8_t* weight_code
   }
   const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n;
   const int64_t pairs = tiles < sms / 2 ? tiles : sms / 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(2 * pairs), 1, 1);
-  cfg.blockDim = dim3(kI8Threads, 1, 1);
-  cfg.dynamicSmemBytes = Cfg::kSmemBytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, int8_linear_pair_kernel<kBf16>, map_a, map_b, map_b16, p);
-  if (e != cudaSuccess) return cuda_fail(e, "8-bit linear (pair) launch");
-  return FMM_OK;
+  return launch_int8(int8_linear_pair_kernel<kBf16>, "8-bit linear (pair) launch", 2 * pairs, kI8Threads,
+                     Cfg::kSmemBytes, 2, stream, map_a, map_b, map_b16, p);
 }
 
 constexpr size_t kI8FewShared = 216 * 1024;
@@ -1351,10 +1356,7 @@ int launch_int8_few(Int8FewParams p, int sms, cudaStream_t stream) {
   const int64_t units = ceil_div(p.N, R);
   p.units = static_cast<int32_t>(units);
   const int grid = static_cast<int>(units < sms ? units : sms);
-  kernel<<<grid, 32 * warps, shared, stream>>>(p);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return cuda_fail(e, "8-bit linear (few tokens) launch");
-  return FMM_OK;
+  return launch_int8(kernel, "8-bit linear (few tokens) launch", grid, 32 * warps, shared, 1, stream, p);
 }
 
 // Channels of a unit of the few-token kernel: the most (4, 2, 1) that leave an

@@ -75,13 +75,15 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const void* tmap, uint
       : "memory");
 }
 
-// D[tmem] (+)= A[smem] * B[smem]^T in 32-bit integers, one elected thread.
-__device__ __forceinline__ void tc_mma_i8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                         uint32_t accumulate) {
+// D[tmem] (+)= A[smem] * B[smem]^T in 32-bit integers, by the lane where
+// `leader` holds.  The whole warp comes here: operands that are the same in
+// every lane stay in uniform registers, where the instruction reads them.
+__device__ __forceinline__ void tc_mma_i8(uint32_t leader, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                         uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
 }
 
@@ -348,15 +350,18 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     prefetch_tmap(&tmap_b);
     if (kTokens) prefetch_tmap(&tmap_c);
   }
+  let_next_kernel_start();
   if (warp == 0) {
     // the ring is filled while tensor memory is being allocated
     __syncwarp();
+    wait_for_previous_kernel();
     while (issued < p.stages && load_t < total && load_ok) load_stage_next();
   }
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), 2 * p.tmem_cols);
     tmem_relinquish();
   }
+  wait_for_previous_kernel();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -391,18 +396,17 @@ __global__ void __launch_bounds__(kI8Threads, 1)
         ok = __all_sync(0xffffffffu, mbar_wait_bounded(full_bar + 8 * stage, phase, abort, p.timeout_ns, 23));
         if (!ok) break;
         tc_fence_after();
-        if (elect_one()) {
-          const int atoms = min(p.atoms, columns - kb);
-          uint64_t b_desc = b_desc0 + stage * stage_step, a_desc = a_desc0 + stage * stage_step;
-          for (int at = 0; at < atoms; ++at) {
+        const int atoms = min(p.atoms, columns - kb);
+        const uint32_t leader = elect_one();
+        uint64_t b_desc = b_desc0 + stage * stage_step, a_desc = a_desc0 + stage * stage_step;
+        for (int at = 0; at < atoms; ++at) {
 #pragma unroll
-            for (int kk = 0; kk < kI8BlockK / 32; ++kk)  // 32 codes on, 32 bytes on
-              tc_mma_i8(d_tmem, a_desc + kk * 2, b_desc + kk * 2, idesc, (kb > 0 || at > 0 || kk > 0) ? 1u : 0u);
-            b_desc += atom_step;
-            a_desc += atom_step;
-          }
-          tc_commit(empty_bar + 8 * stage);
+          for (int kk = 0; kk < kI8BlockK / 32; ++kk)  // 32 codes on, 32 bytes on
+            tc_mma_i8(leader, d_tmem, a_desc + kk * 2, b_desc + kk * 2, idesc, (kb > 0 || at > 0 || kk > 0) ? 1u : 0u);
+          b_desc += atom_step;
+          a_desc += atom_step;
         }
+        if (leader) tc_commit(empty_bar + 8 * stage);
         __syncwarp();
         issued_any = true;
         if (++stage == p.stages) {
@@ -527,6 +531,8 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     tmem_alloc_pair(smem_u32(tmem_slot), 2 * Cfg::kTile);
     tmem_relinquish_pair();
   }
+  let_next_kernel_start();
+  wait_for_previous_kernel();
   tc_fence_before();
   cluster_sync_all();  // barriers of both CTAs initialised, TMEM allocated
   tc_fence_after();
@@ -768,6 +774,8 @@ __global__ void __launch_bounds__(32 * kI8FewMaxWarps, 1) int8_linear_few_kernel
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncwarp();
+  let_next_kernel_start();
+  wait_for_previous_kernel();
   for (int s = 0; s < p.stages; ++s) copy(s);
   // the tokens, zero past K
   for (int i = threadIdx.x; i < p.M * (pitch / 16); i += blockDim.x) {

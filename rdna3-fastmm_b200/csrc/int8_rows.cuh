@@ -32,6 +32,17 @@
 
 namespace fmm {
 
+// Launches of the 8-bit kernels overlap the end of the kernel before them in
+// the stream (programmatic stream serialisation): a CTA may be set up early, and
+// waits here until that kernel has finished and its writes can be seen.  Every
+// thread calls it before it reads or writes global memory, and before any wait
+// with a limit, which would count the other kernel's time.
+__device__ __forceinline__ void wait_for_previous_kernel() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// From here on the next kernel's CTAs may be set up where there is room.
+__device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;"); }
+
 constexpr int kRowsMaxThreads = 1024;
 constexpr int kRowsNormThreads = 768;  // streamed norms: 80 registers a thread (65536 x 4608: 349 us with 64, 333)
 
@@ -248,6 +259,8 @@ __global__ void __launch_bounds__(kRowsMaxThreads, 1) int8_rows_kernel(const Int
   auto first = [&](int v) { return kVec ? (v * width + t) * 8 : v * 8 * width + t; };
   const int loops = V > 0 ? V : (cols + 8 * width - 1) / (8 * width);
   if (kPair && threadIdx.x < 2) s_exact[threadIdx.x] = 0;
+  let_next_kernel_start();
+  wait_for_previous_kernel();
 
   int parity = 0;
   for (int64_t row = int64_t(blockIdx.x) * rows_per_block + (block_row ? 0 : warp); row < p.rows;
@@ -508,10 +521,14 @@ __global__ void __launch_bounds__(kVec && kNorm ? kRowsNormThreads : kRowsMaxThr
     if (a.count > 0) bulk_load(dst + origin(x) + a.head * sizeof(T), x + a.head, a.count * sizeof(T), bar);
     if (b.count > 0) bulk_load(dst + slot + origin(r) + b.head * sizeof(T), r + b.head, b.count * sizeof(T), bar);
   };
+  let_next_kernel_start();
   if (t == 0) {
     s_abort[group] = 0;
     for (int s = 0; s < p.stages; ++s) mbar_init(full_bar + 8 * s, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  wait_for_previous_kernel();
+  if (t == 0) {
     for (int s = 0; s < p.stages; ++s)
       if (row0 + s * row_step < p.rows) fetch(row0 + s * row_step, s);
   }

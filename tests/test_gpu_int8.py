@@ -481,6 +481,42 @@ def test_calls_follow_the_current_stream():
     assert torch.equal(got, expected)
 
 
+@pytest.mark.parametrize("rows", [1, 3, 40, 700])
+def test_back_to_back_calls_wait_for_each_other(rows):
+    """Launches overlap the kernel before them; every buffer here is written by
+    one call and read, then overwritten, by the next ones."""
+    inner = 2048
+    plan = Int8Plan(rows, inner, inner, DEVICE)
+    packed = [plan.pack_weight(_randn((inner, inner), k, BF16, 0.05).to(DEVICE), 0.1) for k in range(3)]
+    gain = (1 + 0.1 * _randn((inner,), 9)).to(BF16).to(DEVICE)
+
+    def run(wait):
+        ws = plan.allocate_workspace(0.1)
+        weight, x = torch.empty((inner, inner), device=DEVICE), _randn((rows, inner), 7, BF16).to(DEVICE)
+        stream = torch.zeros_like(x)
+        wc, wscale = empty_codes((inner, inner), DEVICE), torch.empty(inner, device=DEVICE)
+        for k in range(30):
+            if k % 5:
+                rms_norm_int8(x, gain, stream, codes=ws.codes, scales=ws.scales, residual_out=stream)
+            else:
+                quantize_rows(x, codes=ws.codes, scales=ws.scales)
+            wait()
+            linear_int8(ws.codes, ws.scales, packed[k % 3].codes, packed[k % 3].scales, out=x)
+            wait()
+            weight.fill_(0.001 * k)  # a kernel of another library in between
+            weight.diagonal().add_(x[0].float())
+            quantize_rows(weight, codes=wc, scales=wscale)  # a weight that the next call reads at once
+            wait()
+            linear_int8(ws.codes, ws.scales, wc, wscale, out=x)
+            wait()
+        return x.clone(), stream.clone()
+
+    expected = run(torch.cuda.synchronize)
+    for _ in range(3):
+        got = run(lambda: None)
+        assert torch.equal(got[0], expected[0]) and torch.equal(got[1], expected[1])
+
+
 def test_torch_operators_match_and_compile():
     x, r = _randn((2, 9, 100), 1, BF16).to(DEVICE), _randn((2, 9, 100), 2, BF16).to(DEVICE)
     weight = torch.ones(100, dtype=BF16, device=DEVICE)
