@@ -25,7 +25,7 @@ namespace fmm {
 
 constexpr int kI8Lanes = 128;    // MMA rows of an SM's tile
 constexpr int kI8BlockK = 128;   // k of one 128-byte swizzle row
-constexpr int kI8EpilogueWarps = 8;  // two for each 32 TMEM lanes, every other 32 columns each
+constexpr int kI8EpilogueWarps = 8;  // at most; two for each 32 TMEM lanes, every other 32 columns each
 constexpr int kI8Threads = 64 + 32 * kI8EpilogueWarps;
 constexpr int kI8MaxStages = 24;
 
@@ -204,14 +204,14 @@ __device__ __forceinline__ void store_block(const void* tmap, uint32_t buffer, c
 }
 
 // One accumulator of 128 lanes x `columns` (of them `count` exist) at t_addr,
-// by one epilogue warp: its 32 lanes, every other 32 columns from `first` on.
-// lane0: what the warp's first lane stands for; column0: what column 0 does.
+// by one epilogue warp: its 32 lanes, blocks of 32 columns.  row: what the lane
+// stands for; column0: what column 0 does.
 template <bool kBf16, bool kTokens>
 struct Int8Epilogue {
   const Int8LinearParams& p;
   const void* tmap_c;
   uint32_t buffers;  // kTokens: two blocks of this warp
-  int lane, first;
+  int lane, first, step;  // columns first, first + step, ... in blocks of 32
   int turn = 0;
 
   // scale and bias of lane's row, and the scale (and bias) of column first + lane
@@ -236,11 +236,11 @@ struct Int8Epilogue {
   }
   __device__ __forceinline__ void drain(uint32_t t_addr, int64_t row, int64_t column0, int count) {
 #pragma unroll 1
-    for (int c = first; c < count; c += 64) {
+    for (int c = first; c < count; c += step) {
       uint32_t v[32];
       tc_ld_32x32b_x32(t_addr + c, v);
       const float scale = col_scale, bias = col_bias;
-      load_column(column0, c + 64, count);  // the next ones, before these are waited for
+      load_column(column0, c + step, count);  // the next ones, before these are waited for
       tc_wait_ld();
       if constexpr (kTokens) {
         if (row - lane < p.M)  // the warp's first token
@@ -431,7 +431,8 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   } else {
     const int quarter = warp & 3;  // TMEM lanes this warp may access
     const int block = warp - 2;
-    Int8Epilogue<kBf16, kTokens> epilogue{p, &tmap_c, blocks + block * 2 * kI8BlockBytes, lane, block / 4 * 32};
+    Int8Epilogue<kBf16, kTokens> epilogue{p, &tmap_c, blocks + block * 2 * kI8BlockBytes, lane, block / 4 * 32,
+                                           kI8EpilogueWarps / 4 * 32};
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int t = blockIdx.x; t < total; t += gridDim.x) {
@@ -509,6 +510,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
 
   const int warp = threadIdx.x / 32;
   const int lane = threadIdx.x % 32;
+  const int epilogue_warps = blockDim.x / 32 - 2;  // 4 or 8
   const uint32_t cta = cluster_cta_rank();  // 0 = even CTA (issues the MMAs)
   const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
   if (threadIdx.x == 0) {
@@ -518,7 +520,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(tfull_bar + 8 * b, 1);
-      mbar_init(tempty_bar + 8 * b, 2 * kI8EpilogueWarps);  // of both CTAs
+      mbar_init(tempty_bar + 8 * b, 2 * epilogue_warps);  // of both CTAs
     }
     mbar_init(drain_bar, 1);
     *abort = 0;
@@ -651,7 +653,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   } else {
     const int quarter = warp & 3;
     const uint32_t tempty_even = map_to_cta(tempty_bar, 0);
-    Int8Epilogue<kBf16, false> epilogue{p, nullptr, 0u, lane, (warp - 2) / 4 * 32};
+    Int8Epilogue<kBf16, false> epilogue{p, nullptr, 0u, lane, (warp - 2) / 4 * 32, epilogue_warps / 4 * 32};
     int acc = 0;
     uint32_t acc_phase = 0;
     for (int t = pair; t < total; t += pairs) {
