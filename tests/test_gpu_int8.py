@@ -58,12 +58,14 @@ def _norm_reference(x, weight, residual, eps):
 
 
 def _norm_roundings(inner):
-    # a thread adds 8 V squares one after another (V the vectors of its row),
-    # ten halvings join a block; the root halves what the mean is off, four
-    # roundings follow (mean + eps counts in the sum; root, two quotients, peak)
-    vectors = -(-inner // 8)
-    mine = 8 * max(-(-vectors // 1024), 4)
-    return (mine + 12) / 2 + 4
+    # a thread adds at most 96 squares one after another (12 vectors of 8 of a
+    # streamed row; 8 V = 32 of a row in registers; of a longer row 8 a pass of
+    # 1024 threads), then up to 12 joins (two chains, 5 in the warp, up to 32
+    # warps in 5 or, one after another, 16 warps that share fewer squares); the
+    # root halves what the mean is off, four roundings follow (mean and epsilon,
+    # root, two quotients; the peak is exact or one rounding more)
+    mine = max(96, 8 * -(-inner // 8192))
+    return (mine + 12) / 2 + 5
 
 
 @pytest.mark.parametrize("gain", ["same", "fp32"])
@@ -135,7 +137,8 @@ def test_rows_of_zeros_infinities_and_nans(inner):
 @pytest.mark.parametrize("with_residual", [False, True])
 @pytest.mark.parametrize("gain", ["same", "fp32"])
 @pytest.mark.parametrize("rows,inner", [(12001, 512), (11003, 1024), (4097, 1032), (1201, 4608), (700, 8200), (401, 16384),
-                                        (330, 24576), (310, 32768), (333, 4607)])
+                                        (330, 24576), (310, 32768), (3100, 4607), (9000, 1031), (1300, 9001),
+                                        (20000, 259)])
 def test_many_rows_stream_through(rows, inner, gain, with_residual):
     """More rows than resident blocks take at once; padding rows among them."""
     x = _randn((rows, inner), 1, BF16).to(DEVICE)
@@ -226,9 +229,45 @@ def test_rows_in_larger_buffers(offset, pitch, inner):
     assert bool((o_buf == 9.0).all()) and bool((q_buf == 99).all())
 
 
+@pytest.mark.parametrize("offset,pitch,code_pitch", [(1, 2003, 2000), (3, 2001, 2003), (8, 2008, 2008), (4, 2004, 2016),
+                                                     (5, 2008, 2001)])
+@pytest.mark.parametrize("dtype", [FP16, FP32])
+def test_many_rows_in_larger_buffers(offset, pitch, code_pitch, dtype):
+    """The streamed form at any step and alignment; what lies beside the rows stays."""
+    rows, inner = 6000, 2000
+    cut = lambda b, p: b.view(-1)[offset:offset + rows * p].view(rows, p)[:, :inner]  # noqa: E731
+    x_buf = _randn((rows + 1, pitch), 1, dtype).to(DEVICE)
+    q_buf = torch.full((rows + 1, code_pitch), 99, dtype=torch.int8, device=DEVICE)
+    x, q = cut(x_buf, pitch), cut(q_buf, code_pitch)
+    scales = torch.empty(rows, device=DEVICE)
+    quantize_rows(x, codes=q, scales=scales)
+    expected, peak = _codes(x.double())
+    assert torch.equal(q, expected.to(torch.int8))
+    assert bool(((scales.double() - peak / 127.0).abs() <= U32 * peak / 127.0).all())
+    if dtype != FP32:
+        r_buf = _randn((rows + 1, pitch + 2), 2, dtype).to(DEVICE)
+        o_buf = torch.full((rows + 1, pitch + 1), 9.0, dtype=dtype, device=DEVICE)
+        r, o = cut(r_buf, pitch + 2), cut(o_buf, pitch + 1)
+        weight = (1 + 0.1 * _randn((inner,), 4)).to(DEVICE)
+        rms_norm_int8(x, weight, r, codes=q, scales=scales, residual_out=o)
+        h, p, rstd = _norm_reference(x, weight, r, 1e-6)
+        expected, peak = _codes(p)
+        assert torch.equal(q, expected.to(torch.int8)) and torch.equal(o, h)
+        reference = peak * rstd / 127.0
+        assert bool(((scales.double() - reference).abs() <= _norm_roundings(inner) * U32 * reference).all())
+        expected_stream = o.clone()
+        rms_norm_int8(x, weight, r, codes=q, scales=scales, residual_out=r)  # in place
+        assert torch.equal(r, expected_stream) and torch.equal(q, expected.to(torch.int8))
+        o.fill_(9.0)
+        assert bool((o_buf == 9.0).all())
+    q.fill_(99)
+    assert bool((q_buf == 99).all())
+
+
+@pytest.mark.parametrize("rows", [6, 4000])
 @pytest.mark.parametrize("inner", [96, 4608, 40000])
-def test_the_stream_is_updated_in_place(inner):
-    x, r = _randn((6, inner), 1, FP16).to(DEVICE), _randn((6, inner), 2, FP16).to(DEVICE)
+def test_the_stream_is_updated_in_place(inner, rows):
+    x, r = _randn((rows, inner), 1, FP16).to(DEVICE), _randn((rows, inner), 2, FP16).to(DEVICE)
     weight = torch.ones(inner, device=DEVICE)
     expected = rms_norm_int8(x, weight, r)
     for target in ("residual", "x"):
