@@ -1102,16 +1102,22 @@ template <class T, class G, bool kNorm, bool kVec>
 int dispatch_int8_rows(Int8RowsParams p, const DeviceInfo* info, cudaStream_t stream) {
   const int64_t vectors = ceil_div(p.cols, 8);
   const int64_t row_bytes = p.cols * int64_t(sizeof(T));
-  if (row_bytes >= 512 && (!kVec || row_bytes % 16 == 0)) {
-    const size_t slot = static_cast<size_t>(round_up(row_bytes, 16)) + (kVec ? 0 : 16);
-    const size_t code_bytes = kVec ? 0 : static_cast<size_t>(round_up(p.cols, 16));
-    Int8RowsParams streamed = p;
+  if (row_bytes >= 512) {
+    // the streamed form takes vectors of 8 elements where rows are whole ones
+    // (FP32 rows of 4 n elements are aligned, but need not be), else elements
+    const bool whole = kVec && p.cols % 8 == 0;
+    const size_t slot = static_cast<size_t>(round_up(row_bytes, 16)) + (whole ? 0 : 16);
+    const size_t code_bytes = whole ? 0 : static_cast<size_t>(round_up(p.cols, 16));
     const size_t gain_bytes = kNorm ? static_cast<size_t>(round_up(p.cols * int64_t(4), 16)) : 0;
+    Int8RowsParams streamed = p;
     if (plan_streamed_rows(&streamed, slot, code_bytes, gain_bytes) &&
         p.rows > 2 * int64_t(usable_sms(info)) * streamed.groups) {
       const size_t shared =
           gain_bytes + streamed.groups * (streamed.stages * slot * (p.residual != nullptr ? 2 : 1) + code_bytes);
-      return launch_int8_rows_streamed<T, G, kNorm, kVec>(streamed, shared, info, stream);
+      if constexpr (kVec) {
+        if (whole) return launch_int8_rows_streamed<T, G, kNorm, true>(streamed, shared, info, stream);
+      }
+      return launch_int8_rows_streamed<T, G, kNorm, false>(streamed, shared, info, stream);
     }
   }
   if (vectors <= 128) {

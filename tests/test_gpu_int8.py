@@ -264,6 +264,23 @@ def test_many_rows_in_larger_buffers(offset, pitch, code_pitch, dtype):
     assert bool((q_buf == 99).all())
 
 
+@pytest.mark.parametrize("rows,inner,dtype", [(20000, 300, FP32), (3100, 4612, FP32), (9000, 1004, FP32), (5, 4612, FP32),
+                                              (20000, 132, FP32), (12000, 260, BF16), (9000, 1001, FP16)])
+def test_aligned_rows_that_are_not_whole_vectors(rows, inner, dtype):
+    """FP32 rows of 4 n elements, and 16-bit rows of any length at an aligned step."""
+    pitch = inner if dtype == FP32 else -(-inner // 8) * 8
+    x = _randn((rows, pitch), 1, dtype).to(DEVICE)[:, :inner]
+    codes, scales = quantize_rows(x)
+    expected, peak = _codes(x.double())
+    assert torch.equal(codes, expected.to(torch.int8))
+    assert bool(((scales.double() - peak / 127.0).abs() <= U32 * peak / 127.0).all())
+    if dtype != FP32:
+        weight = (1 + 0.1 * _randn((inner,), 4)).to(dtype).to(DEVICE)
+        codes, scales, h = rms_norm_int8(x, weight, x)
+        reference, p, _ = _norm_reference(x, weight, x, 1e-6)
+        assert torch.equal(codes, _codes(p)[0].to(torch.int8)) and torch.equal(h, reference)
+
+
 @pytest.mark.parametrize("rows", [6, 4000])
 @pytest.mark.parametrize("inner", [96, 4608, 40000])
 def test_the_stream_is_updated_in_place(inner, rows):
