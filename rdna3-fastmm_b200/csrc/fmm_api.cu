@@ -1418,7 +1418,9 @@ int launch_linear_int8(const int8_t* codes, int64_t ldq, const int8_t* weight_co
     if (p.M == 2) return launch_int8_few_tokens<kBf16, 2>(f, channels, sms, stream);
     return launch_int8_few_tokens<kBf16, 4>(f, channels, sms, stream);
   }
-  const bool rows16 = aligned(p.out, 16) && p.ldc % 8 == 0;
+  // a box store ends at a whole 16 bytes of a row: a row that ends inside them
+  // would take up to 7 of the elements behind it along
+  const bool rows16 = aligned(p.out, 16) && p.ldc % 8 == 0 && p.N % 8 == 0;
   const Int8Shape shape = choose_int8_shape(p.M, p.K, p.N, rows16, sms);
   if (shape.pair) return launch_int8_pair<kBf16>(codes, ldq, weight_codes, ldw, p, sms, stream);
   return shape.tokens ? launch_int8_single<kBf16, true>(codes, ldq, weight_codes, ldw, p, shape, sms, stream)

@@ -154,7 +154,9 @@ __device__ __forceinline__ void store_columns(const Int8LinearParams& p, const u
   }
 }
 
-// Tiled TMA store (shared -> global) of one box; what lies outside is not written.
+// Tiled TMA store (shared -> global) of one box.  Rows outside are not written,
+// nor 16-byte units of a row; the unit that holds a row's end is written whole,
+// so the host takes this form for rows of whole units.
 __device__ __forceinline__ void tma_store_2d(const void* tmap, uint32_t src, int32_t c0, int32_t c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(
                    reinterpret_cast<uint64_t>(tmap)),

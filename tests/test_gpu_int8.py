@@ -417,6 +417,20 @@ def test_linear_writes_its_output_only(rows, columns):
         assert bool((buf == 7.0).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,columns,pitch", [(1167, 329, 352), (14595, 9, 16), (2083, 2574, 2592), (113, 13975, 13984),
+                                                (2610, 1, 16), (5389, 13, 32), (464, 6271, 6272), (2083, 2568, 2592)])
+def test_linear_writes_columns_of_a_larger_buffer(rows, columns, pitch, dtype):
+    """Aligned rows, whose last 16 bytes hold columns of somebody else."""
+    a, w = (torch.randint(-127, 128, (n, 48), device=DEVICE, dtype=torch.int8) for n in (rows, columns))
+    sa = torch.rand(rows, device=DEVICE) * 0.01 + 1e-3
+    sw = torch.rand(columns, device=DEVICE) * 1e-3 + 1e-4
+    buffer = torch.full((rows, pitch), 7.0, device=DEVICE, dtype=dtype)
+    linear_int8(a, sa, w, sw, out=buffer[:, :columns])
+    assert torch.equal(buffer[:, :columns], linear_int8(a, sa, w, sw, dtype=dtype))
+    assert (buffer[:, columns:] == 7.0).all()
+
+
 def test_linear_reads_code_rows_of_any_pitch():
     rows, inner, columns = 20, 200, 150
     case = _linear_case(rows, inner, columns, FP16, False)
