@@ -1094,15 +1094,18 @@ int launch_int8_rows_streamed(Int8RowsParams p, size_t shared, const DeviceInfo*
                      32 * p.warps_per_row * p.groups, shared, 1, stream, p);
 }
 
-// Many rows are streamed.  Otherwise a row of up to 1024 elements is one
-// warp's (four vectors of 8 a lane), four rows a block; longer rows are a
-// block's, with the fewest vectors a thread that 1024 threads cover; beyond
-// 32768 elements the row is read twice.
+// Many rows of more than one vector a lane are streamed (65536 BF16 rows, us
+// streamed and from registers: 256 elements 23.5, 18.7; 512: 29.7, 31.3; 1024:
+// 42.1, 49.0; norm of 256 with a residual 39.9, 33.4; FP32 rows of 256: 22.7,
+// 18.8).  Otherwise a row of up to 1024 elements is one warp's (four vectors of
+// 8 a lane), four rows a block; longer rows are a block's, with the fewest
+// vectors a thread that 1024 threads cover; beyond 32768 elements the row is
+// read twice.
 template <class T, class G, bool kNorm, bool kVec>
 int dispatch_int8_rows(Int8RowsParams p, const DeviceInfo* info, cudaStream_t stream) {
   const int64_t vectors = ceil_div(p.cols, 8);
   const int64_t row_bytes = p.cols * int64_t(sizeof(T));
-  if (row_bytes >= 512) {
+  if (vectors > 32) {
     // the streamed form takes vectors of 8 elements where rows are whole ones
     // (FP32 rows of 4 n elements are aligned, but need not be), else elements
     const bool whole = kVec && p.cols % 8 == 0;
