@@ -167,6 +167,13 @@ def _refuse_grad(*tensors: torch.Tensor | None) -> None:
             raise ValueError("the B200 8-bit operators do not support autograd")
 
 
+def _refuse_negated(*tensors: torch.Tensor | None) -> None:
+    """The storage of a lazily negated view (``z.conj().imag``) holds the other sign."""
+    for tensor in tensors:
+        if tensor is not None and tensor.is_neg():
+            raise ValueError("lazily negated views must be resolved (torch.resolve_neg) first")
+
+
 def _require_cuda(tensor: torch.Tensor, name: str) -> int:
     device = tensor.get_device()
     if device < 0 or not tensor.is_cuda:
@@ -258,6 +265,7 @@ def quantize_rows(x: torch.Tensor, *, codes: torch.Tensor | None = None,
         raise ValueError("x must have a last dimension of at least one element")
     if _grad_enabled():
         _refuse_grad(x, codes, scales)
+    _refuse_negated(x, codes, scales)
     held, source = _input_rows(x)
     leading = shape[:-1]
     if codes is None:
@@ -302,6 +310,7 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
         raise ValueError("residual_out needs a residual")
     if _grad_enabled():
         _refuse_grad(x, weight, residual, codes, scales, residual_out)
+    _refuse_negated(x, weight, residual, codes, scales, residual_out)
     held, source = _input_rows(x)
     if not weight.is_contiguous():
         weight = weight.contiguous()
@@ -370,6 +379,7 @@ def linear_int8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.T
         raise ValueError(f"linear_int8 writes BF16 or FP16, not {dtype}")
     if _grad_enabled():
         _refuse_grad(scales, weight_scales, bias, out)
+    _refuse_negated(codes, scales, weight_codes, weight_scales, bias, out)
     q, w = _flat(codes), _flat(weight_codes)
     if q is None or w is None:
         raise ValueError("codes must have dense rows a constant step apart")
@@ -527,6 +537,7 @@ class Int8Plan:
         """What the product would refuse, before the first kernel has changed anything."""
         buffers = [_input_rows(buffer)[1] for buffer in (workspace.codes, workspace.scales)]
         packed = [_input_rows(tensor)[1] for tensor in (weight.codes, weight.scales)]
+        _refuse_negated(bias, output)
         if any(_rows_overlap(buffer, tensor) for buffer in buffers for tensor in packed):
             raise ValueError("work buffers must not overlap")
         if bias is not None:

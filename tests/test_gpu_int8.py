@@ -716,3 +716,37 @@ def test_plan_refusals():
     out = other.run_linear_packed(torch.ones((6, 64), dtype=BF16, device=DEVICE), packed,
                                   other.allocate_workspace(0.1))
     assert out.shape == (6, 8)  # a packed weight serves other row counts
+
+
+def test_negated_views_are_refused():
+    """Their storage holds the other sign; the torch operators are given resolved ones."""
+    z = torch.randn(5, 64, device=DEVICE, dtype=torch.complex64)
+    x = z.conj().imag
+    assert x.is_neg()
+    rows = x.resolve_neg()
+    codes, scales = quantize_rows(rows)
+    assert torch.equal(torch.ops.rdna3_fastmm.quantize_rows_int8(x)[0], codes)
+    half = rows.to(FP16)
+    gain, neg = torch.ones(64, device=DEVICE, dtype=FP16), torch._neg_view
+    w, ws = quantize_rows(torch.randn(24, 64, device=DEVICE))
+    bias, out = torch.ones(24, device=DEVICE, dtype=FP16), torch.zeros(5, 24, device=DEVICE, dtype=FP16)
+    plan = Int8Plan(5, 64, 24, torch.device(DEVICE), FP16)
+    packed, workspace = plan.pack_weight(rows.new_ones(24, 64)), plan.allocate_workspace()
+    workspace.codes.fill_(3)
+    for call in (lambda: quantize_rows(x),
+                 lambda: quantize_rows(rows, scales=neg(scales.clone())),
+                 lambda: rms_norm_int8(neg(half), gain),
+                 lambda: rms_norm_int8(half, neg(gain)),
+                 lambda: rms_norm_int8(half, gain, neg(half)),
+                 lambda: rms_norm_int8(half, gain, half, residual_out=neg(half.clone())),
+                 lambda: linear_int8(codes, neg(scales), w, ws),
+                 lambda: linear_int8(codes, scales, w, neg(ws)),
+                 lambda: linear_int8(codes, scales, w, ws, neg(bias)),
+                 lambda: linear_int8(codes, scales, w, ws, out=neg(out)),
+                 lambda: plan.run_linear_packed(neg(half), packed, workspace),
+                 lambda: plan.run_linear_packed(half, packed, workspace, neg(bias)),
+                 lambda: plan.run_linear_packed(half, packed, workspace, output=neg(out))):
+        with pytest.raises(ValueError, match="negated"):
+            call()
+    assert (workspace.codes == 3).all()
+    assert (out == 0).all()
