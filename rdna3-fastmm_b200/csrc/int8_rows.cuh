@@ -704,10 +704,20 @@ __global__ void __launch_bounds__(kVec && kNorm ? kRowsNormThreads : kRowsMaxThr
 
     // ---- codes
     if (!scale.plain) {
-      for (int c = t; c < cols; c += width) {
-        const int8_t byte = settled_code(scale.zero ? 0.0 : exact(c), exact_peak, scale);
-        if constexpr (kVec) q[c] = byte;
-        else s_codes[c] = byte;
+      // elements as above: with a residual the stage holds sums that only the
+      // thread which wrote them is sure to see (a group of one warp has no
+      // barrier in between)
+      if constexpr (kVec) {
+        for (int c = 8 * t; c < cols; c += 8 * width) {
+          uint64_t eight = 0;
+#pragma unroll 1
+          for (int e = 0; e < (scale.zero ? 0 : 8); ++e)
+            eight |= static_cast<uint64_t>(static_cast<uint8_t>(settled_code(exact(c + e), exact_peak, scale))) << (8 * e);
+          *reinterpret_cast<uint64_t*>(q + c) = eight;
+        }
+      } else {
+        for (int c = t; c < cols; c += width)
+          s_codes[c] = settled_code(scale.zero ? 0.0 : exact(c), exact_peak, scale);
       }
     } else if constexpr (kVec) {
 #pragma unroll 4
