@@ -352,7 +352,6 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     prefetch_tmap(&tmap_b);
     if (kTokens) prefetch_tmap(&tmap_c);
   }
-  let_next_kernel_start();
   if (warp == 0) {
     // the ring is filled while tensor memory is being allocated
     __syncwarp();
@@ -367,6 +366,10 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Behind the barrier that follows the allocation: a CTA of the next kernel
+  // allocates before it waits for this one, and must not take the columns first
+  // if it ever fits beside this CTA.
+  let_next_kernel_start();
   const uint32_t tmem_base = *tmem_slot;
 
   if (warp == 0) {
@@ -535,11 +538,11 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     tmem_alloc_pair(smem_u32(tmem_slot), 2 * Cfg::kTile);
     tmem_relinquish_pair();
   }
-  let_next_kernel_start();
   wait_for_previous_kernel();
   tc_fence_before();
   cluster_sync_all();  // barriers of both CTAs initialised, TMEM allocated
   tc_fence_after();
+  let_next_kernel_start();  // behind the allocation, as above
   const uint32_t tmem_base = *tmem_slot;
 
   const int total = p.tiles_m * p.tiles_n;

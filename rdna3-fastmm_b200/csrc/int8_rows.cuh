@@ -40,7 +40,8 @@ namespace fmm {
 __device__ __forceinline__ void wait_for_previous_kernel() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
-// From here on the next kernel's CTAs may be set up where there is room.
+// From here on the next kernel's CTAs may be set up where there is room; a kernel
+// with tensor memory calls it once its own allocation is made.
 __device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;"); }
 
 constexpr int kRowsMaxThreads = 1024;
