@@ -122,6 +122,20 @@ def _input_rows(tensor: torch.Tensor) -> tuple[torch.Tensor, _Rows]:
     return tensor, (tensor.data_ptr(), *flat, tensor.element_size())
 
 
+def _touched_rows(tensor: torch.Tensor) -> _Rows:
+    """The rows of a tensor where it lies, for checks of overlap: of one whose
+    rows are not dense, rows that hold its elements (no copy is made)."""
+    flat = _flat(tensor)
+    if flat is None:
+        *inside, (pitch, rows) = sorted((stride, size) for size, stride in zip(tensor.shape, tensor.stride()) if size != 1)
+        inner = 1 + sum(stride * (size - 1) for stride, size in inside)
+        if pitch < inner:
+            rows, inner = min(rows, 1), inner + pitch * (rows - 1)
+            pitch = inner
+        flat = rows if tensor.numel() else 0, inner, pitch
+    return tensor.data_ptr(), *flat, tensor.element_size()
+
+
 def _output_rows(tensor: torch.Tensor, shape: torch.Size, dtype: torch.dtype, device: int, name: str,
                  like: _Rows | None = None) -> _Rows:
     if tensor.shape != shape:
@@ -535,11 +549,9 @@ class Int8Plan:
     def _validate_product(self, workspace: Int8Workspace, weight: Int8PackedWeight, bias: torch.Tensor | None,
                           output: torch.Tensor | None) -> None:
         """What the product would refuse, before the first kernel has changed anything."""
-        buffers = [_input_rows(buffer)[1] for buffer in (workspace.codes, workspace.scales)]
-        packed = [_input_rows(tensor)[1] for tensor in (weight.codes, weight.scales)]
+        buffers = [_touched_rows(buffer) for buffer in (workspace.codes, workspace.scales)]
+        read = [_touched_rows(tensor) for tensor in (weight.codes, weight.scales)]
         _refuse_negated(bias, output)
-        if any(_rows_overlap(buffer, tensor) for buffer in buffers for tensor in packed):
-            raise ValueError("work buffers must not overlap")
         if bias is not None:
             if tuple(bias.shape) != (self.columns,):
                 raise ValueError(f"bias matrix has shape {tuple(bias.shape)}, expected {(self.columns,)}")
@@ -547,13 +559,15 @@ class Int8Plan:
                 raise ValueError("bias matrix device or dtype does not match the plan")
             if _grad_enabled():
                 _refuse_grad(bias)
+            read.append(_touched_rows(bias))
+        # the first kernel writes the buffers before the product reads the others
+        if any(_rows_overlap(buffer, tensor) for buffer in buffers for tensor in read):
+            raise ValueError("work buffers must not overlap")
         if output is not None:
             rows = _output_rows(output, torch.Size((self.rows, self.columns)), self.dtype, self.device.index, "output")
             if _grad_enabled():
                 _refuse_grad(output)
-            if bias is not None:
-                packed.append(_input_rows(bias)[1])
-            if any(_rows_overlap(rows, tensor) for tensor in buffers + packed):
+            if any(_rows_overlap(rows, tensor) for tensor in buffers + read):
                 raise ValueError("output storage must not overlap inputs or workspace")
 
     @staticmethod
@@ -561,9 +575,9 @@ class Int8Plan:
         """What the first kernel reads or writes must outlive the second's output."""
         if output is None or _flat(output) is None:
             return  # a malformed output is refused where it is used
-        rows = _input_rows(output)[1]
+        rows = _touched_rows(output)
         for tensor in tensors:
-            if tensor is not None and _rows_overlap(rows, _input_rows(tensor)[1]):
+            if tensor is not None and _rows_overlap(rows, _touched_rows(tensor)):
                 raise ValueError("output storage must not overlap inputs or workspace")
 
 
