@@ -18,8 +18,8 @@ code is ``code * scale``; codes are symmetric, ``round(127 x / max|x|)``.
 Code rows start on 16-byte boundaries: a ``[rows, K]`` tensor of codes made
 here is a view of ``[rows, round_up(K, 16)]`` storage.  Calls are queued on the
 current stream of the operands' device; with buffers given for their outputs
-they allocate nothing and capture into CUDA graphs.  They do not support
-autograd: an operand that requires a gradient is refused while gradients are
+they allocate nothing and capture into CUDA graphs; autograd sees such buffers as
+changed in place.  The operators do not support autograd themselves: an operand that requires a gradient is refused while gradients are
 enabled.  The reference has no quantised operator.
 """
 
@@ -77,6 +77,7 @@ _BF16, _FP16, _FP32, _INT8 = torch.bfloat16, torch.float16, torch.float32, torch
 _grad_enabled = torch.is_grad_enabled
 _current_device = torch._C._cuda_getDevice
 _current_stream = torch._C._cuda_getCurrentRawStream
+_mark_written = torch.autograd.graph.increment_version  # of buffers given, as by any operator that writes in place
 _ROW_TYPES = {torch.bfloat16: _native.FMM_DTYPE_BF16, torch.float16: _native.FMM_DTYPE_F16,
               torch.float32: _native.FMM_DTYPE_F32}
 
@@ -282,6 +283,7 @@ def quantize_rows(x: torch.Tensor, *, codes: torch.Tensor | None = None,
     _refuse_negated(x, codes, scales)
     held, source = _input_rows(x)
     leading = shape[:-1]
+    given = [tensor for tensor in (codes, scales) if tensor is not None]
     if codes is None:
         codes = empty_codes(shape, x.device)
     if scales is None:
@@ -293,6 +295,8 @@ def quantize_rows(x: torch.Tensor, *, codes: torch.Tensor | None = None,
     _refuse_overlap([q, s], [source])
     if rows:
         _launch(device, "fmm_quantize_rows", dtype, *source[:4], q[0], q[3], s[0])
+        if given:
+            _mark_written(given)
     return Int8Rows(codes, scales)
 
 
@@ -331,6 +335,7 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
     ptr, rows, inner, pitch, _ = source
     gain = weight.data_ptr(), 1, inner, inner, 4 if gain_kind is _FP32 else 2
     leading = shape[:-1]
+    given = [tensor for tensor in (codes, scales, residual_out) if tensor is not None]
     if codes is None:
         codes = empty_codes(shape, x.device)
     if scales is None:
@@ -343,6 +348,8 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
         if rows:
             _launch(device, "fmm_rms_norm_int8", _ROW_TYPES[kind], _ROW_TYPES[gain_kind], ptr, pitch, None, 0, gain[0],
                     rows, inner, eps, None, 0, q[0], q[3], s[0])
+            if given:
+                _mark_written(given)
         return NormedInt8Rows(codes, scales, None)
     if residual.shape != shape or residual.dtype is not kind or residual.get_device() != device:
         raise ValueError("residual must have x's shape, dtype and device")
@@ -361,6 +368,8 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
     if rows:
         _launch(device, "fmm_rms_norm_int8", _ROW_TYPES[kind], _ROW_TYPES[gain_kind], ptr, pitch, added[0], added[3],
                 gain[0], rows, inner, eps, stream[0], stream[3], q[0], q[3], s[0])
+        if given:
+            _mark_written(given)
     return NormedInt8Rows(codes, scales, residual_out)
 
 
@@ -408,6 +417,7 @@ def linear_int8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.T
     rows, _, pitch = q
     ptr, weight_ptr, bias_ptr = codes.data_ptr(), weight_codes.data_ptr(), None if bias is None else bias.data_ptr()
     scales_ptr, weight_scales_ptr = scales.data_ptr(), weight_scales.data_ptr()
+    given = out
     if out is None:
         out = torch.empty((*leading, columns), device=codes.device, dtype=dtype)
         result_ptr, result_pitch = out.data_ptr(), columns if rows > 1 else (columns + 15) & -16
@@ -423,6 +433,8 @@ def linear_int8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.T
     if rows:
         _launch(device, "fmm_linear_int8", _ROW_TYPES[dtype], ptr, pitch, scales_ptr, weight_ptr, w[2],
                 weight_scales_ptr, bias_ptr, result_ptr, result_pitch, rows, inner, columns)
+        if given is not None:
+            _mark_written(given)
     return out
 
 
