@@ -19,8 +19,10 @@ Code rows start on 16-byte boundaries: a ``[rows, K]`` tensor of codes made
 here is a view of ``[rows, round_up(K, 16)]`` storage.  Calls are queued on the
 current stream of the operands' device; with buffers given for their outputs
 they allocate nothing and capture into CUDA graphs; autograd sees such buffers as
-changed in place.  The operators do not support autograd themselves: an operand that requires a gradient is refused while gradients are
-enabled.  The reference has no quantised operator.
+changed in place.  The operators do not support autograd themselves: an operand
+that requires a gradient is refused while gradients are enabled, one with a
+forward-mode tangent always, and ``torch.func`` transforms are refused too.  The
+reference has no quantised operator.
 """
 
 from __future__ import annotations
@@ -29,6 +31,8 @@ from dataclasses import dataclass
 from typing import NamedTuple, Optional
 
 import torch
+from torch._functorch import eager_transforms
+from torch.autograd import forward_ad
 
 from . import _native
 from .runtime import _LinearPlan, _round_up
@@ -77,7 +81,7 @@ _BF16, _FP16, _FP32, _INT8 = torch.bfloat16, torch.float16, torch.float32, torch
 _grad_enabled = torch.is_grad_enabled
 _current_device = torch._C._cuda_getDevice
 _current_stream = torch._C._cuda_getCurrentRawStream
-_mark_written = torch.autograd.graph.increment_version  # of buffers given, as by any operator that writes in place
+_mark_written = torch._C._increment_version  # of buffers given, as by any operator that writes in place
 _ROW_TYPES = {torch.bfloat16: _native.FMM_DTYPE_BF16, torch.float16: _native.FMM_DTYPE_F16,
               torch.float32: _native.FMM_DTYPE_F32}
 
@@ -175,18 +179,26 @@ def _output_scales(tensor: torch.Tensor, shape: torch.Size, device: int) -> None
         raise ValueError(f"scales must be contiguous float32 on cuda:{device}")
 
 
-def _refuse_grad(*tensors: torch.Tensor | None) -> None:
-    """Called while gradients are enabled."""
+def _refuse_unread(*tensors: torch.Tensor | None) -> None:
+    """Refuse what the storage alone does not hold: a gradient to come, a
+    forward-mode tangent, the other sign of a lazily negated view (``z.conj().imag``)."""
+    grad = _grad_enabled()
     for tensor in tensors:
-        if tensor is not None and tensor.requires_grad:
-            raise ValueError("the B200 8-bit operators do not support autograd")
+        if tensor is not None:
+            if grad and tensor.requires_grad:
+                raise ValueError("the B200 8-bit operators do not support autograd")
+            if tensor.is_neg():
+                raise ValueError("lazily negated views must be resolved (torch.resolve_neg) first")
+    if forward_ad._current_level >= 0:
+        for tensor in tensors:
+            if tensor is not None and forward_ad.unpack_dual(tensor).tangent is not None:
+                raise ValueError("the B200 8-bit operators do not support autograd")
 
 
-def _refuse_negated(*tensors: torch.Tensor | None) -> None:
-    """The storage of a lazily negated view (``z.conj().imag``) holds the other sign."""
-    for tensor in tensors:
-        if tensor is not None and tensor.is_neg():
-            raise ValueError("lazily negated views must be resolved (torch.resolve_neg) first")
+def _refuse_transforms() -> None:
+    """Of the torch operators: ``torch.func.jvp`` takes the tangents off before they get here."""
+    if eager_transforms.JVP_NESTING > 0:
+        raise ValueError("the B200 8-bit operators do not support torch.func.jvp")
 
 
 def _require_cuda(tensor: torch.Tensor, name: str) -> int:
@@ -278,16 +290,18 @@ def quantize_rows(x: torch.Tensor, *, codes: torch.Tensor | None = None,
     shape = x.shape
     if len(shape) < 1 or shape[-1] < 1:
         raise ValueError("x must have a last dimension of at least one element")
-    if _grad_enabled():
-        _refuse_grad(x, codes, scales)
-    _refuse_negated(x, codes, scales)
+    _refuse_unread(x, codes, scales)
     held, source = _input_rows(x)
     leading = shape[:-1]
-    given = [tensor for tensor in (codes, scales) if tensor is not None]
+    given = ()
     if codes is None:
         codes = empty_codes(shape, x.device)
+    else:
+        given = (codes,)
     if scales is None:
         scales = torch.empty(leading, device=x.device, dtype=torch.float32)
+    else:
+        given += (scales,)
     q = _output_rows(codes, shape, _INT8, device, "codes", source)
     _output_scales(scales, leading, device)
     rows = source[1]
@@ -326,20 +340,22 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
         raise ValueError("eps must be finite and not negative")
     if residual is None and residual_out is not None:
         raise ValueError("residual_out needs a residual")
-    if _grad_enabled():
-        _refuse_grad(x, weight, residual, codes, scales, residual_out)
-    _refuse_negated(x, weight, residual, codes, scales, residual_out)
+    _refuse_unread(x, weight, residual, codes, scales, residual_out)
     held, source = _input_rows(x)
     if not weight.is_contiguous():
         weight = weight.contiguous()
     ptr, rows, inner, pitch, _ = source
     gain = weight.data_ptr(), 1, inner, inner, 4 if gain_kind is _FP32 else 2
     leading = shape[:-1]
-    given = [tensor for tensor in (codes, scales, residual_out) if tensor is not None]
+    given = () if residual_out is None else (residual_out,)
     if codes is None:
         codes = empty_codes(shape, x.device)
+    else:
+        given += (codes,)
     if scales is None:
         scales = torch.empty(leading, device=x.device, dtype=torch.float32)
+    else:
+        given += (scales,)
     q = _output_rows(codes, shape, _INT8, device, "codes", source)
     _output_scales(scales, leading, device)
     s = scales.data_ptr(), 1 if rows else 0, rows, rows, 4
@@ -400,9 +416,7 @@ def linear_int8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.T
         dtype = out.dtype if out is not None else bias.dtype if bias is not None else torch.bfloat16
     if dtype is not _BF16 and dtype is not _FP16:
         raise ValueError(f"linear_int8 writes BF16 or FP16, not {dtype}")
-    if _grad_enabled():
-        _refuse_grad(scales, weight_scales, bias, out)
-    _refuse_negated(codes, scales, weight_codes, weight_scales, bias, out)
+    _refuse_unread(codes, scales, weight_codes, weight_scales, bias, out)
     q, w = _flat(codes), _flat(weight_codes)
     if q is None or w is None:
         raise ValueError("codes must have dense rows a constant step apart")
@@ -434,7 +448,7 @@ def linear_int8(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.T
         _launch(device, "fmm_linear_int8", _ROW_TYPES[dtype], ptr, pitch, scales_ptr, weight_ptr, w[2],
                 weight_scales_ptr, bias_ptr, result_ptr, result_pitch, rows, inner, columns)
         if given is not None:
-            _mark_written(given)
+            _mark_written((given,))
     return out
 
 
@@ -563,22 +577,18 @@ class Int8Plan:
         """What the product would refuse, before the first kernel has changed anything."""
         buffers = [_touched_rows(buffer) for buffer in (workspace.codes, workspace.scales)]
         read = [_touched_rows(tensor) for tensor in (weight.codes, weight.scales)]
-        _refuse_negated(bias, output)
+        _refuse_unread(bias, output)
         if bias is not None:
             if tuple(bias.shape) != (self.columns,):
                 raise ValueError(f"bias matrix has shape {tuple(bias.shape)}, expected {(self.columns,)}")
             if bias.device != self.device or bias.dtype != self.dtype:
                 raise ValueError("bias matrix device or dtype does not match the plan")
-            if _grad_enabled():
-                _refuse_grad(bias)
             read.append(_touched_rows(bias))
         # the first kernel writes the buffers before the product reads the others
         if any(_rows_overlap(buffer, tensor) for buffer in buffers for tensor in read):
             raise ValueError("work buffers must not overlap")
         if output is not None:
             rows = _output_rows(output, torch.Size((self.rows, self.columns)), self.dtype, self.device.index, "output")
-            if _grad_enabled():
-                _refuse_grad(output)
             if any(_rows_overlap(rows, tensor) for tensor in buffers + read):
                 raise ValueError("output storage must not overlap inputs or workspace")
 
@@ -596,6 +606,7 @@ class Int8Plan:
 # ---------------------------------------------------------------- torch.library
 @torch.library.custom_op("rdna3_fastmm::quantize_rows_int8", mutates_args=(), device_types="cuda")
 def quantize_rows_int8_op(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    _refuse_transforms()
     codes, scales = quantize_rows(x)
     return codes, scales
 
@@ -603,6 +614,7 @@ def quantize_rows_int8_op(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 @torch.library.custom_op("rdna3_fastmm::rms_norm_int8", mutates_args=(), device_types="cuda")
 def rms_norm_int8_op(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None,
                      eps: float = 1e-6) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    _refuse_transforms()
     codes, scales, stream = rms_norm_int8(x, weight, residual, eps)
     # without a residual there is no new one: an operator cannot return None
     return codes, scales, x.new_empty((0,)) if stream is None else stream
@@ -612,6 +624,7 @@ def rms_norm_int8_op(x: torch.Tensor, weight: torch.Tensor, residual: Optional[t
 def linear_int8_op(codes: torch.Tensor, scales: torch.Tensor, weight_codes: torch.Tensor,
                    weight_scales: torch.Tensor, bias: Optional[torch.Tensor] = None,
                    dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    _refuse_transforms()
     return linear_int8(codes, scales, weight_codes, weight_scales, bias, dtype=dtype)
 
 

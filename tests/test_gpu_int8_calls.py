@@ -1,7 +1,8 @@
-"""What the 8-bit operators tell autograd."""
+"""What the 8-bit operators tell autograd, and what they refuse of it."""
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from rdna3_fastmm.int8 import Int8Plan, empty_codes, linear_int8, quantize_rows, rms_norm_int8
 
@@ -75,3 +76,39 @@ def test_buffers_of_inference_mode():
         got = quantize_rows(x, codes=codes, scales=scales)
     again = quantize_rows(x, codes=codes, scales=scales)
     assert again.codes is codes and torch.equal(got.codes, again.codes)
+
+
+def test_tangents_are_refused():
+    """A dual tensor does not require a gradient, and its tangent would be lost without a word."""
+    x, gain, tangent = _randn(5, 64), torch.ones(64, device=DEVICE), _randn(5, 64)
+    codes, scales = quantize_rows(x)
+    w, ws = quantize_rows(_randn(8, 64))
+    bias, out = _randn(8), torch.zeros((5, 8), dtype=BF16, device=DEVICE)
+    plan = Int8Plan(5, 64, 8, DEVICE)
+    packed, workspace = plan.pack_weight(_randn(8, 64), 0.1), plan.allocate_workspace(0.1)
+    operators = torch.ops.rdna3_fastmm
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: quantize_rows(dual(x)),
+                     lambda: rms_norm_int8(dual(x), gain),
+                     lambda: rms_norm_int8(x, dual(gain)),
+                     lambda: rms_norm_int8(x, gain, dual(x)),
+                     lambda: linear_int8(codes, dual(scales), w, ws),
+                     lambda: linear_int8(codes, scales, w, dual(ws)),
+                     lambda: linear_int8(codes, scales, w, ws, dual(bias)),
+                     lambda: linear_int8(codes, scales, w, ws, out=dual(out)),
+                     lambda: plan.run_linear_packed(dual(x), packed, workspace),
+                     lambda: plan.run_linear_packed(x, packed, workspace, dual(bias)),
+                     lambda: plan.run_norm_linear_packed(x, dual(gain), packed, workspace),
+                     lambda: operators.quantize_rows_int8(dual(x)),
+                     lambda: operators.rms_norm_int8(dual(x), gain),
+                     lambda: operators.linear_int8(codes, dual(scales), w, ws)):
+            with torch.no_grad(), pytest.raises(ValueError, match="autograd"):
+                call()
+        rms_norm_int8(x, gain)  # operands without one
+        operators.linear_int8(codes, scales, w, ws)
+    for function in (quantize_rows, operators.quantize_rows_int8, lambda x: rms_norm_int8(x, gain),
+                     lambda x: operators.rms_norm_int8(x, gain)):
+        with pytest.raises((ValueError, RuntimeError)):
+            torch.func.jvp(lambda x: function(x)[1], (x,), (tangent,))
+    assert not out.any()

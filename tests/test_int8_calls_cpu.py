@@ -5,6 +5,7 @@ from pathlib import Path
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from rdna3_fastmm import int8
 
@@ -79,3 +80,37 @@ def test_rows_of_tensors_that_are_not_dense():
     # beside each other in the rows of one buffer
     assert not int8._rows_overlap(int8._touched_rows(buffer[:, :10:2]), int8._touched_rows(buffer[:, 10:]))
     assert int8._rows_overlap(int8._touched_rows(buffer[:, :12:2]), int8._touched_rows(buffer[:, 10:]))
+
+
+def test_gradients_tangents_and_negated_views_are_refused():
+    x, codes = torch.zeros(3, 4), torch.zeros((3, 4), dtype=torch.int8)
+    int8._refuse_unread(x, None, codes)
+    leaf = x.clone().requires_grad_(True)
+    for refused in (leaf, leaf * 2, torch._neg_view(x), torch._neg_view(codes)):
+        with pytest.raises(ValueError):
+            int8._refuse_unread(x, None, refused)
+    with torch.no_grad():
+        int8._refuse_unread(leaf, leaf * 2)
+    with forward_ad.dual_level():
+        int8._refuse_unread(x, codes)
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for operand in (dual, dual * 2, dual.t()):
+            with pytest.raises(ValueError, match="autograd"):
+                int8._refuse_unread(x, operand)
+            with torch.no_grad(), pytest.raises(ValueError, match="autograd"):  # which leaves tangents alone
+                int8._refuse_unread(x, operand)
+    int8._refuse_unread(x)
+
+
+def test_torch_operators_refuse_forward_transforms():
+    def call(x):
+        int8._refuse_transforms()
+        return x
+
+    x = torch.zeros(3)
+    torch.func.vmap(call)(x)
+    torch.func.grad(lambda x: call(x).sum())(x)
+    for transform in (lambda: torch.func.jvp(call, (x,), (x,)), lambda: torch.func.jacfwd(call)(x)):
+        with pytest.raises(ValueError, match="jvp"):
+            transform()
+    call(x)
