@@ -11,14 +11,15 @@
 //
 // Codes are those of exact arithmetic.  p is exact in FP32 where x and g have
 // 16 bits (at most 22 significant bits); with an FP32 gain the threads that
-// hold the largest rounded p look its FP64 value up.  127 / a is rounded, so
+// hold the largest rounded p look its FP64 value up.  Rows whose products leave
+// FP32's range, below or above, are taken once more in FP64 (take_row_wide).  127 / a is rounded, so
 // each product is taken by the FP32 numbers on either side of it; where the
 // two codes differ (1 product in 10^5), 254 p and (2c + 1) a are compared in
 // FP64, exact on both sides.
 //
-// A row with an infinity or a NaN (or, in the norm, with a square beyond FP32)
-// has codes 0 and a NaN scale: whatever is computed from it is NaN.  A row of
-// zeros has codes 0 and scale 0.
+// A row with an infinity or a NaN (or, in the norm, with a square or a scale
+// beyond FP32) has codes 0 and a NaN scale: whatever is computed from it is NaN.
+// A row of zeros has codes 0 and scale 0.
 //
 // Two kernels.  Few rows: a block (or a warp) a row, the row in registers, for
 // the shortest way from the first byte to the last.  Many rows: bound by HBM,
@@ -147,36 +148,32 @@ __device__ __forceinline__ RowTotals warp_totals(RowTotals t) {
 // computed from both sides: by `low` and by `high`, a few steps of FP32 apart
 // with the exact quotient between them.  Where both give the same code it is
 // the exact one; where they differ, the product is next to a border.  Rows that
-// are not plain (zeros, not finite, or so small or large that 127 / a leaves
-// FP32) take settled_code for every element, lifted into range.
+// are not plain are zeros, not finite, or so small or large that FP32's products,
+// 127 / a or the scale lose digits.
 struct RowScale {
-  bool finite, zero;  // zero: all codes are 0
   bool plain;
-  float lift;
   float low, high;
 };
 // kPair: the product and the peak are rounded too
 template <bool kNorm, bool kPair>
 __device__ __forceinline__ RowScale row_scale(const RowTotals& total) {
   RowScale s;
-  s.finite = total.peak < 0x7f800000u && (!kNorm || __float_as_uint(total.square) < 0x7f800000u);
-  s.zero = !s.finite || total.peak == 0u;
   const float peak = __uint_as_float(total.peak);
-  s.plain = !s.zero && peak >= 0x1p-100f && peak <= 0x1p100f;
-  s.lift = peak < 0x1p-100f ? 0x1p100f : peak > 0x1p100f ? 0x1p-100f : 1.0f;
+  // false for NaN; a norm's scale, at most 2^50 a / 127, stays in FP32
+  s.plain = peak >= 0x1p-100f && peak <= (kNorm ? 0x1p50f : 0x1p100f);
+  if (kNorm) s.plain = s.plain && __float_as_uint(total.square) < 0x7f800000u;
   // the quotient is at most half a step off, the pair's other two roundings a step more each
   constexpr uint32_t kSteps = kPair ? 3 : 1;
-  const uint32_t middle = __float_as_uint(127.0f / (s.zero ? 1.0f : peak * s.lift));
+  const uint32_t middle = __float_as_uint(127.0f / peak);
   s.low = __uint_as_float(middle - kSteps);
   s.high = __uint_as_float(middle + kSteps);
   return s;
 }
 template <bool kNorm>
-__device__ __forceinline__ float stored_scale(const RowTotals& total, const RowScale& s, int cols, float eps) {
+__device__ __forceinline__ float stored_scale(const RowTotals& total, int cols, float eps) {
   float scale = __uint_as_float(total.peak);
-  // a row of zeros has scale 0, without an epsilon too
-  if (kNorm && total.peak != 0u) scale = scale / sqrtf(total.square / static_cast<float>(cols) + eps);
-  return s.finite ? scale / 127.0f : __uint_as_float(0x7fc00000u);
+  if (kNorm) scale = scale / sqrtf(total.square / static_cast<float>(cols) + eps);
+  return scale / 127.0f;
 }
 
 // x + kMagic rounds x to an integer, the low byte of the sum: no conversions,
@@ -225,13 +222,76 @@ __device__ __forceinline__ uint4 add_vec(float (&h)[8], const float (&f)[8]) {
   return w;
 }
 
-// The code of a product next to a border or of a row that is not plain, P its
-// FP64 value.
+// The code of a plain row's product next to a border, P its FP64 value.
 __device__ __forceinline__ int8_t settled_code(double P, double exact_peak, const RowScale& s) {
-  if (s.zero) return 0;
-  const double lifted = P * s.lift;
-  const int below = static_cast<int>(floorf(static_cast<float>(lifted) * s.low));
-  return static_cast<int8_t>(exact_code(lifted, exact_peak * s.lift, below));
+  const int below = static_cast<int>(floorf(static_cast<float>(P) * s.low));
+  return static_cast<int8_t>(exact_code(P, exact_peak, below));
+}
+
+// round_half_even(127 P / M) without a guess at hand, 0 < M, |P| <= M.  The floor may
+// be one off next to an integer: both codes that it leaves are looked at.
+__device__ __forceinline__ int8_t wide_code(double P, double M) {
+  return static_cast<int8_t>(exact_code(P, M, static_cast<int>(floor(127.0 * P / M))));
+}
+
+// One row in FP64, where its products are exact (48 bits at most, between 2^-282
+// and 2^256), by the `width` threads that had it: a warp, or those of named
+// barrier `barrier` with a word of `squares` and `peaks` for each warp.  Reads
+// h, the stream in memory, in the order in which its own threads wrote it.
+template <class T, class G, bool kNorm, bool kVec>
+__device__ __forceinline__ void take_row_wide(const T* h, const G* gain, int8_t* codes, float* scale, int cols, float eps,
+                                              int t, int width, int barrier, double* squares, unsigned long long* peaks) {
+  constexpr int kRun = kVec ? 8 : 1;  // consecutive elements of a thread
+  auto product = [&](int c) {
+    double P = static_cast<double>(RowVec<T>::one(h + c));
+    if constexpr (kNorm) P *= static_cast<double>(RowVec<G>::one(gain + c));
+    return P;
+  };
+  double square = 0.0;
+  unsigned long long bits = 0;  // of the largest |p|, which compare as the values do, NaN above infinities
+#pragma unroll 1
+  for (int c0 = kRun * t; c0 < cols; c0 += kRun * width)
+#pragma unroll 1
+    for (int c = c0; c < min(c0 + kRun, cols); ++c) {
+      const float v = RowVec<T>::one(h + c);
+      if (kNorm) {
+        // a square beyond FP32 makes the row one that is not finite
+        const float low = v * v;
+        square += __float_as_uint(low) < 0x7f800000u ? static_cast<double>(v) * v : static_cast<double>(low);
+      }
+      const unsigned long long mine = static_cast<unsigned long long>(__double_as_longlong(fabs(product(c))));
+      bits = mine > bits ? mine : bits;
+    }
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    square += __shfl_xor_sync(0xffffffffu, square, d);
+    bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, d));
+  }
+  if (width > 32) {
+    if (t % 32 == 0) {
+      squares[t / 32] = square;
+      peaks[t / 32] = bits;
+    }
+    named_barrier_sync(barrier, width);
+    square = 0.0;
+#pragma unroll 1
+    for (int w = 0; w < width / 32; ++w) {
+      square += squares[w];
+      bits = max(bits, peaks[w]);
+    }
+    named_barrier_sync(barrier, width);  // the next row writes them
+  }
+  const double peak = __longlong_as_double(static_cast<long long>(bits));
+  double s = peak / 127.0;
+  if (kNorm && peak > 0.0) s /= sqrt(square / cols + static_cast<double>(eps));
+  // a scale beyond FP32 is not finite either
+  const bool finite = s <= static_cast<double>(3.402823466e38f) && (!kNorm || square < static_cast<double>(INFINITY));
+  const bool zero = !finite || peak == 0.0;
+  if (t == 0) *scale = finite ? static_cast<float>(s) : __uint_as_float(0x7fc00000u);
+#pragma unroll 1
+  for (int c0 = kRun * t; c0 < cols; c0 += kRun * width)
+#pragma unroll 1
+    for (int c = c0; c < min(c0 + kRun, cols); ++c) codes[c] = zero ? 0 : wide_code(product(c), peak);
 }
 
 // ---------------------------------------------------------------- few rows
@@ -247,6 +307,8 @@ __global__ void __launch_bounds__(kRowsMaxThreads, 1) int8_rows_kernel(const Int
   __shared__ float s_square[2][32];
   __shared__ uint32_t s_peak[2][32];
   __shared__ unsigned long long s_exact[2];
+  __shared__ double s_wide_square[32];
+  __shared__ unsigned long long s_wide_peak[32];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const bool block_row = p.warps_per_row > 1;
   const int rows_per_block = block_row ? 1 : blockDim.x / 32;
@@ -318,10 +380,14 @@ __global__ void __launch_bounds__(kRowsMaxThreads, 1) int8_rows_kernel(const Int
       }
     };
     float square = 0.0f, most = 0.0f;
+    uint32_t seen = 0;  // of the bits of h
     auto take = [&](int v, float (&h)[8]) {
       if constexpr (kNorm) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) square = fmaf(h[e], h[e], square);
+        for (int e = 0; e < 8; ++e) {
+          square = fmaf(h[e], h[e], square);
+          seen |= __float_as_uint(h[e]);
+        }
       }
       times_gain(v, h);
 #pragma unroll
@@ -361,12 +427,41 @@ __global__ void __launch_bounds__(kRowsMaxThreads, 1) int8_rows_kernel(const Int
       total = warp_totals<kNorm>(total);
     }
     const RowScale scale = row_scale<kNorm, kPair>(total);
-    if (t == 0) p.scales[row] = stored_scale<kNorm>(total, scale, cols, p.eps);
+    if (kNorm && !scale.plain) {
+      // a row of zeros has codes 0 and scale 0, without an epsilon too; its
+      // products may be 0 without it
+      bool zeros = total.peak == 0u;
+      if (zeros) {
+        const bool mine_zero = (seen & 0x7fffffffu) == 0;
+        zeros = block_row ? named_barrier_and(0, width, mine_zero) : __all_sync(0xffffffffu, mine_zero);
+      }
+      if (!zeros) {
+        take_row_wide<T, G, kNorm, kVec>(stream, gain, q, p.scales + row, cols, p.eps, t, width, 0, s_wide_square,
+                                         s_wide_peak);
+      } else {
+        if (t == 0) p.scales[row] = 0.0f;
+#pragma unroll 1
+        for (int v = 0; v < loops; ++v) {
+          const int c0 = first(v);
+          if (kVec && c0 + 8 <= cols) {
+            *reinterpret_cast<uint2*>(q + c0) = make_uint2(0u, 0u);
+            continue;
+          }
+#pragma unroll 1
+          for (int c = c0; c < min(c0 + 8 * step, cols); c += step) q[c] = 0;
+        }
+      }
+      if (kPair && block_row && threadIdx.x == 0) s_exact[parity ^ 1] = 0;  // as below
+      parity ^= 1;
+      continue;
+    }
+    const bool finite = kNorm || total.peak < 0x7f800000u;
+    if (t == 0) p.scales[row] = finite ? stored_scale<kNorm>(total, cols, p.eps) : __uint_as_float(0x7fc00000u);
     double exact_peak = __uint_as_float(total.peak);
     if constexpr (kPair) {
       // p is rounded here: those who hold the largest look it up in FP64
       unsigned long long bits = 0;
-      if (mine == total.peak && scale.finite) {
+      if (mine == total.peak) {
         double value = 0.0;
         if constexpr (V > 0) {
           uint32_t largest = 0;
@@ -407,9 +502,14 @@ __global__ void __launch_bounds__(kRowsMaxThreads, 1) int8_rows_kernel(const Int
         read(v, stream, nullptr, held[0]);
         times_gain(v, held[0]);
       }
-      if (!scale.plain) {
-        for (int c = c0; c < min(c0 + 8 * step, cols); c += step)
-          q[c] = settled_code(scale.zero ? 0.0 : exact(c), exact_peak, scale);
+      if (!kNorm && !scale.plain) {
+        // without a norm the peak is exact, and codes are all that is left
+        const bool zero = !finite || total.peak == 0u;
+        if (kVec && zero && c0 + 8 <= cols) {
+          *reinterpret_cast<uint2*>(q + c0) = make_uint2(0u, 0u);
+          continue;
+        }
+        for (int c = c0; c < min(c0 + 8 * step, cols); c += step) q[c] = zero ? 0 : wide_code(exact(c), exact_peak);
         continue;
       }
       float code[8], other[8];
@@ -434,6 +534,28 @@ __global__ void __launch_bounds__(kRowsMaxThreads, 1) int8_rows_kernel(const Int
 }
 
 // ---------------------------------------------------------------- many rows
+// The scale of a streamed row that waits for take_row_wide, a NaN that nothing
+// computes.  Such rows are rare, and are taken behind the loop over the rows:
+// inside it, the registers cost the others 5 to 10 % (8214 x 4608: 39.7 us, 44.8).
+constexpr uint32_t kRowWaits = 0x7fffffffu;
+// It finds its place from the parameters: nothing of the loop's stays in registers for it.
+template <class T, class G, bool kNorm, bool kVec>
+__device__ __noinline__ void take_waiting_rows(const Int8RowsParams& p) {
+  __shared__ double squares[32];
+  __shared__ unsigned long long peaks[32];
+  const int width = p.warps_per_row * 32, group = threadIdx.x / width, t = threadIdx.x - group * width;
+  const bool add = kNorm && p.residual != nullptr;
+  if (width == 32) __syncwarp();
+  else named_barrier_sync(1 + group, width);
+  for (int64_t row = int64_t(group) * gridDim.x + blockIdx.x; row < p.rows; row += int64_t(gridDim.x) * p.groups) {
+    if (*reinterpret_cast<const volatile uint32_t*>(p.scales + row) != kRowWaits) continue;
+    const T* stream = add ? static_cast<const T*>(p.residual_out) + row * p.ldo : static_cast<const T*>(p.x) + row * p.ldx;
+    take_row_wide<T, G, kNorm, kVec>(stream, static_cast<const G*>(p.gain), p.codes + row * p.ldq, p.scales + row, p.cols,
+                                     p.eps, t, width, 1 + group, squares + group * p.warps_per_row,
+                                     peaks + group * p.warps_per_row);
+  }
+}
+
 // Bulk copy of 16-byte units (both addresses aligned) into this CTA's shared
 // memory, completing on the mbarrier at `bar`.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -473,7 +595,7 @@ constexpr int kRowsMaxStages = 4;
 // apart, and codes are collected in shared memory.
 template <class T, class G, bool kNorm, bool kVec>
 __global__ void __launch_bounds__(kVec && kNorm ? kRowsNormThreads : kRowsMaxThreads, 1)
-    int8_rows_streamed_kernel(const Int8RowsParams p) {
+    int8_rows_streamed_kernel(const __grid_constant__ Int8RowsParams p) {
   constexpr bool kPair = kNorm && std::is_same<G, float>::value;
   __shared__ __align__(8) uint64_t s_full[kRowsMaxGroups * kRowsMaxStages];
   __shared__ float s_square[kRowsMaxGroups];
@@ -551,6 +673,7 @@ __global__ void __launch_bounds__(kVec && kNorm ? kRowsNormThreads : kRowsMaxThr
 
   int stage = 0;
   uint32_t phase = 0;
+  bool waits = false;  // some row is left to take_row_wide
   for (int64_t row = row0; row < p.rows; row += row_step) {
     int8_t* q = p.codes + row * p.ldq;
     T* ro = add ? static_cast<T*>(p.residual_out) + row * p.ldo : nullptr;
@@ -663,7 +786,7 @@ __global__ void __launch_bounds__(kVec && kNorm ? kRowsNormThreads : kRowsMaxThr
                    : *static_cast<volatile int*>(&s_abort[group]) != 0)
       break;
     const RowScale scale = row_scale<kNorm, kPair>(total);
-    if (t == 0) p.scales[row] = stored_scale<kNorm>(total, scale, cols, p.eps);
+    if (scale.plain && t == 0) p.scales[row] = stored_scale<kNorm>(total, cols, p.eps);
     // p of one element in FP64, exact
     auto exact = [&](int c) {
       double P = static_cast<double>(RowVec<T>::one(h + c));
@@ -671,10 +794,10 @@ __global__ void __launch_bounds__(kVec && kNorm ? kRowsNormThreads : kRowsMaxThr
       return P;
     };
     double exact_peak = __uint_as_float(total.peak);
-    if constexpr (kPair) {
+    if (kPair && scale.plain) {
       // p is rounded here: those who hold the largest look it up in FP64
       unsigned long long bits = 0;
-      if (mine == total.peak && !scale.zero) {
+      if (mine == total.peak) {
         double value = 0.0;
         auto look = [&](int c0) {
 #pragma unroll
@@ -705,20 +828,33 @@ __global__ void __launch_bounds__(kVec && kNorm ? kRowsNormThreads : kRowsMaxThr
 
     // ---- codes
     if (!scale.plain) {
-      // elements as above: with a residual the stage holds sums that only the
-      // thread which wrote them is sure to see (a group of one warp has no
-      // barrier in between)
-      if constexpr (kVec) {
-        for (int c = 8 * t; c < cols; c += 8 * width) {
-          uint64_t eight = 0;
+      // a row of zeros has codes 0 and scale 0, without an epsilon too; a norm's
+      // products may be 0 without it.  Elements as above: with a residual the
+      // stage holds sums that only the thread which wrote them is sure to see (a
+      // group of one warp has no barrier in between)
+      bool zeros = total.peak == 0u;
+      if (kNorm && zeros) {
+        uint32_t seen = 0;
+        if constexpr (kVec) {
 #pragma unroll 1
-          for (int e = 0; e < (scale.zero ? 0 : 8); ++e)
-            eight |= static_cast<uint64_t>(static_cast<uint8_t>(settled_code(exact(c + e), exact_peak, scale))) << (8 * e);
-          *reinterpret_cast<uint64_t*>(q + c) = eight;
+          for (int c = 8 * t; c < cols; c += 8 * width) {
+            const uint4 v = *reinterpret_cast<const uint4*>(h + c);
+            seen |= (v.x | v.y | v.z | v.w) & 0x7fff7fffu;  // 16-bit elements
+          }
+        } else {
+#pragma unroll 1
+          for (int c = t; c < cols; c += width) seen |= RowVec<T>::one(h + c) != 0.0f ? 1u : 0u;
         }
+        zeros = warps == 1 ? __all_sync(0xffffffffu, seen == 0) : named_barrier_and(1 + group, width, seen == 0);
+      }
+      if (t == 0) p.scales[row] = zeros ? 0.0f : __uint_as_float(kRowWaits);
+      waits = waits || !zeros;
+      if constexpr (kVec) {
+#pragma unroll 1
+        for (int c = 8 * t; c < cols; c += 8 * width) *reinterpret_cast<uint2*>(q + c) = make_uint2(0u, 0u);
       } else {
-        for (int c = t; c < cols; c += width)
-          s_codes[c] = settled_code(scale.zero ? 0.0 : exact(c), exact_peak, scale);
+#pragma unroll 1
+        for (int c = t; c < cols; c += width) s_codes[c] = 0;
       }
     } else if constexpr (kVec) {
 #pragma unroll 4
@@ -782,6 +918,7 @@ __global__ void __launch_bounds__(kVec && kNorm ? kRowsNormThreads : kRowsMaxThr
       if (row0 + s * row_step < p.rows)
         mbar_wait_bounded(full_bar + 8 * s, s < stage ? phase ^ 1u : phase, &no_abort, p.timeout_ns, 32);
   }
+  if (waits) take_waiting_rows<T, G, kNorm, kVec>(p);
 }
 
 }  // namespace fmm

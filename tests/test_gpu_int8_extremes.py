@@ -14,7 +14,7 @@ U32 = 2.0**-24  # half a step of FP32
 
 # rows of a warp or a block in registers, vectors and elements; rows read
 # twice; streamed rows of one warp and of several, vectors and elements
-REGISTERS = [(5, 40), (6, 301), (5, 700), (7, 1001), (5, 5001), (4, 8200), (3, 40000)]
+REGISTERS = [(25, 40), (24, 301), (26, 700), (25, 1001), (24, 5001), (23, 8200), (23, 40000)]
 STREAMED = [(9700, 600), (9700, 601), (3700, 4608), (2700, 4607)]
 FORMS = [(*shape, "int8_rows_kernel") for shape in REGISTERS] + [(*shape, "int8_rows_streamed_kernel")
                                                                  for shape in STREAMED]
@@ -106,3 +106,43 @@ def test_quantised_rows_of_extreme_magnitude(rows, inner, kernel, dtype):
     x = _special(_randn((rows, inner), 1, dtype), values)
     _check(quantize_rows(x), x.double(), None, 0.0, inner)
     assert kernels_of(lambda: quantize_rows(x)) == [kernel]
+
+
+@each
+def test_products_below_the_normal_range(rows, inner, kernel, gain_type, with_residual):
+    """Rows whose products are subnormal numbers of FP32, or less than those."""
+    x = _special(_randn((rows, inner), 3, BF16), [2.0**-70, 2.0**-50, 2.0**-90, 0.0, 2.0**-71, _last(2.0**-60)])
+    residual = x.clone() if with_residual else None
+    gain = ((1 + 0.2 * _randn((inner,), 4)) * 2.0**-77).to(FP32 if gain_type == "fp32" else BF16)
+    _check_norm(x, gain, residual, 1e-6, kernel)
+
+
+@each
+def test_products_beyond_the_range_of_fp32(rows, inner, kernel, gain_type, with_residual):
+    """Finite values times a finite gain, whose norm is finite again."""
+    x = _special(_randn((rows, inner), 7, BF16), [16.0, 0.0, 2.0**-30, 2.0**60, _last(float("inf"))])
+    residual = x.clone() if with_residual else None
+    gain = ((1 + 0.1 * _randn((inner,), 8)).clamp(0.5, 1.5) * 2.0**125).to(FP32 if gain_type == "fp32" else BF16)
+    _check_norm(x, gain, residual, 1e-6, kernel)
+
+
+def test_a_scale_beyond_fp32_is_nan():
+    x = torch.zeros((3, 40000), dtype=BF16, device=DEVICE)
+    x[0, 7], x[1, 3], x[2] = 1.0, -5.0, 1.0
+    gain = torch.full((40000,), torch.finfo(FP32).max, device=DEVICE)
+    codes, scales, _ = rms_norm_int8(x, gain, eps=0.0)  # 200 times the gain, over 127
+    assert scales[:2].isnan().all() and not codes[:2].any()
+    assert bool((codes[2] == 127).all()) and abs(scales[2].item() * 127.0 / torch.finfo(FP32).max - 1) < 4 * U32
+
+
+@pytest.mark.parametrize("gain", [0.0, float("inf"), float("nan")])
+@pytest.mark.parametrize("rows,inner", [(4, 300), (4, 5000), (9700, 600)])
+def test_gains_without_a_value(rows, inner, gain):
+    """A gain of zeros gives zeros; one that is not finite gives rows that are not."""
+    x = _special(_randn((rows, inner), 9, BF16), [0.0, 2.0**-100])
+    weight = torch.zeros(inner, dtype=BF16, device=DEVICE)
+    weight[inner // 2] = gain
+    for eps in (1e-6, 0.0):
+        codes, scales, _ = rms_norm_int8(x, weight, eps=eps)
+        assert not codes.any()
+        assert bool((scales == 0).all()) if gain == 0.0 else bool(scales.isnan().all())
