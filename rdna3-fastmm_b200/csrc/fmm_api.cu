@@ -1685,6 +1685,7 @@ int fmm_rms_norm_int8(int dtype, int gain_dtype, const void* X, int64_t ldx, con
   p.ldq = ldq;
   p.cols = static_cast<int32_t>(cols);
   p.eps = eps;
+  p.eps_sum = eps * static_cast<float>(cols);
   const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (gain_dtype == FMM_DTYPE_F32)
     return dtype == FMM_DTYPE_F16 ? run_int8_rows<__half, float, true>(p, s)

@@ -11,11 +11,11 @@
 //
 // Codes are those of exact arithmetic.  p is exact in FP32 where x and g have
 // 16 bits (at most 22 significant bits); with an FP32 gain the threads that
-// hold the largest rounded p look its FP64 value up.  Rows whose products leave
-// FP32's range, below or above, are taken once more in FP64 (take_row_wide).  127 / a is rounded, so
-// each product is taken by the FP32 numbers on either side of it; where the
-// two codes differ (1 product in 10^5), 254 p and (2c + 1) a are compared in
-// FP64, exact on both sides.
+// hold the largest rounded p look its FP64 value up.  Rows whose products or
+// squares leave FP32's range, below or above, are taken once more in FP64
+// (take_row_wide).  127 / a is rounded, so each product is taken by the FP32
+// numbers on either side of it; where the two codes differ (1 product in 10^5),
+// 254 p and (2c + 1) a are compared in FP64, exact on both sides.
 //
 // A row with an infinity or a NaN (or, in the norm, with a square or a scale
 // beyond FP32) has codes 0 and a NaN scale: whatever is computed from it is NaN.
@@ -59,6 +59,7 @@ struct Int8RowsParams {
   int64_t ldx, ldr, ldo, ldq;
   int32_t cols;
   float eps;
+  float eps_sum;  // eps * cols
   // register form: > 1: the block is one row's; 1: every warp has a row of its own.
   // Streamed form: the warps of a group
   int32_t warps_per_row;
@@ -149,19 +150,25 @@ __device__ __forceinline__ RowTotals warp_totals(RowTotals t) {
 // with the exact quotient between them.  Where both give the same code it is
 // the exact one; where they differ, the product is next to a border.  Rows that
 // are not plain are zeros, not finite, or so small or large that FP32's products,
-// 127 / a or the scale lose digits.
+// squares, 127 / a or the scale lose digits.
 struct RowScale {
   bool plain;
   float low, high;
 };
+// 2^low <= the positive number of these bits < 2^high
+__device__ __forceinline__ bool within(uint32_t bits, int low, int high) {
+  return bits - (static_cast<uint32_t>(low + 127) << 23) < static_cast<uint32_t>(high - low) << 23;
+}
 // kPair: the product and the peak are rounded too
 template <bool kNorm, bool kPair>
-__device__ __forceinline__ RowScale row_scale(const RowTotals& total) {
+__device__ __forceinline__ RowScale row_scale(const RowTotals& total, float eps_sum) {
   RowScale s;
   const float peak = __uint_as_float(total.peak);
   // false for NaN; a norm's scale, at most 2^50 a / 127, stays in FP32
-  s.plain = peak >= 0x1p-100f && peak <= (kNorm ? 0x1p50f : 0x1p100f);
-  if (kNorm) s.plain = s.plain && __float_as_uint(total.square) < 0x7f800000u;
+  s.plain = within(total.peak, -100, kNorm ? 50 : 100);
+  // Squares lose digits below 2^-126, 2^-150 each at most: nothing beside a mean and
+  // epsilon of 2^-100 and more (rows have up to 2^30 elements)
+  if (kNorm) s.plain = s.plain && within(__float_as_uint(total.square + eps_sum), -70, 128);
   // the quotient is at most half a step off, the pair's other two roundings a step more each
   constexpr uint32_t kSteps = kPair ? 3 : 1;
   const uint32_t middle = __float_as_uint(127.0f / peak);
@@ -426,7 +433,7 @@ __global__ void __launch_bounds__(kRowsMaxThreads, 1) int8_rows_kernel(const Int
       total.peak = in ? s_peak[parity][lane] : 0u;
       total = warp_totals<kNorm>(total);
     }
-    const RowScale scale = row_scale<kNorm, kPair>(total);
+    const RowScale scale = row_scale<kNorm, kPair>(total, p.eps_sum);
     if (kNorm && !scale.plain) {
       // a row of zeros has codes 0 and scale 0, without an epsilon too; its
       // products may be 0 without it
@@ -785,7 +792,7 @@ __global__ void __launch_bounds__(kVec && kNorm ? kRowsNormThreads : kRowsMaxThr
     if (warps == 1 ? __any_sync(0xffffffffu, *static_cast<volatile int*>(&s_abort[group]) != 0)
                    : *static_cast<volatile int*>(&s_abort[group]) != 0)
       break;
-    const RowScale scale = row_scale<kNorm, kPair>(total);
+    const RowScale scale = row_scale<kNorm, kPair>(total, p.eps_sum);
     if (scale.plain && t == 0) p.scales[row] = stored_scale<kNorm>(total, cols, p.eps);
     // p of one element in FP64, exact
     auto exact = [&](int c) {

@@ -118,6 +118,16 @@ def test_products_below_the_normal_range(rows, inner, kernel, gain_type, with_re
 
 
 @each
+def test_squares_outside_the_range_of_fp32(rows, inner, kernel, gain_type, with_residual):
+    """Squares that underflow with no epsilon to cover it, and sums of finite squares that overflow."""
+    x = _special(_randn((rows, inner), 5, BF16), [2.0**-76, 2.0**-66, 0.0, 2.0**60, 2.0**-61, 2.0**-100, 2.0**-120])
+    residual = x.clone() if with_residual else None
+    gain = (1 + 0.2 * _randn((inner,), 6)).to(FP32 if gain_type == "fp32" else BF16)
+    _check_norm(x, gain, residual, 0.0, kernel)
+    _check_norm(x, gain, residual, 2.0**-140, kernel)
+
+
+@each
 def test_products_beyond_the_range_of_fp32(rows, inner, kernel, gain_type, with_residual):
     """Finite values times a finite gain, whose norm is finite again."""
     x = _special(_randn((rows, inner), 7, BF16), [16.0, 0.0, 2.0**-30, 2.0**60, _last(float("inf"))])
