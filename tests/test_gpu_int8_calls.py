@@ -15,6 +15,7 @@ def _randn(*shape):
     return torch.randn(shape, device=DEVICE).to(BF16)
 
 
+@torch.enable_grad()  # whatever the mode that a test before left behind
 @pytest.mark.parametrize("target", ["residual", "x"])
 def test_backward_notices_a_stream_that_was_updated_in_place(target):
     """A trainable linear saved the stream; an in-place norm of it, without a gradient of its own, came after."""

@@ -82,6 +82,7 @@ def test_rows_of_tensors_that_are_not_dense():
     assert int8._rows_overlap(int8._touched_rows(buffer[:, :12:2]), int8._touched_rows(buffer[:, 10:]))
 
 
+@torch.enable_grad()  # whatever the mode that a test before left behind
 def test_gradients_tangents_and_negated_views_are_refused():
     x, codes = torch.zeros(3, 4), torch.zeros((3, 4), dtype=torch.int8)
     int8._refuse_unread(x, None, codes)
