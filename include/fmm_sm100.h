@@ -245,8 +245,10 @@ int fmm_quantize_rows(int dtype, const void* X, int64_t rows, int64_t cols, int6
  *   codes and scales of the rows of y, as fmm_quantize_rows of unrounded y
  * dtype (X, residual, residual_out): FMM_DTYPE_BF16 or FMM_DTYPE_F16;
  * gain_dtype: the same, or FMM_DTYPE_F32.  residual_out may be residual or X
- * itself (same address and leading dimension).  A row with a value that is
- * not finite, or whose square is not, has codes 0 and a NaN scale. */
+ * itself (same address and leading dimension).  A row with a value, or a
+ * square of one, that is not finite in FP32, with a gain that is not, or with a
+ * scale beyond FP32 has codes 0 and a NaN scale; sums and products may leave
+ * FP32's range on the way (such rows are taken in FP64). */
 int fmm_rms_norm_int8(int dtype, int gain_dtype, const void* X, int64_t ldx, const void* residual, int64_t ldr,
                       const void* gain, int64_t rows, int64_t cols, float eps, void* residual_out, int64_t ldo,
                       int8_t* codes, int64_t ldq, float* scales, fmm_stream_t stream);

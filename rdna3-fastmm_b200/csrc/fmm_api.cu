@@ -1044,11 +1044,11 @@ constexpr size_t kRowsRingBytes = 216 * 1024;  // rings of the streamed form
 // stages where there is room.  A lane takes about eight vectors of a row, so
 // that the reduction is a small part of its work, but 15 warps are at work at
 // least.  Measured (us, bf16): 16384 elements, three groups of 5, 8, 10 warps
-// 50.9, 45.4, 49.1 (4992 rows); norm of 4608 with residual, five groups of 2,
-// 3, 4, 6 warps 403, 348, 372, 364 (65536 rows); 32768 elements, one group of
-// 12, 16, 24, 32 warps 167, 157, 169, 187 (8192 rows).  Rows that are not
-// aligned have many more instructions: all 32 warps (4607 elements, 1 or 2
-// warps a row: 270, 149).  Returns false where two stages of a row do not fit.
+// 48.2, 43.0, 48.2 (4992 rows); norm of 4608 with residual, five groups of 2,
+// 3, 4, 6 warps 391, 334, 362, 385 (65536 rows); 32768 elements, one group of
+// 12, 16, 24, 32 warps 169, 156, 169, 182 (8192 rows).  Rows that are not
+// aligned have many more instructions: all 32 warps (12288 x 4607 in FP32, five
+// groups of 1, 2, 6 warps: 159, 101, 70).  Returns false where two stages of a row do not fit.
 bool plan_streamed_rows(Int8RowsParams* p, size_t slot, size_t code_bytes, size_t gain_bytes) {
   if (gain_bytes >= kRowsRingBytes) return false;
   const size_t room = kRowsRingBytes - gain_bytes;
@@ -1095,9 +1095,9 @@ int launch_int8_rows_streamed(Int8RowsParams p, size_t shared, const DeviceInfo*
 }
 
 // Many rows of more than one vector a lane are streamed (65536 BF16 rows, us
-// streamed and from registers: 256 elements 23.5, 18.7; 512: 29.7, 31.3; 1024:
-// 42.1, 49.0; norm of 256 with a residual 39.9, 33.4; FP32 rows of 256: 22.7,
-// 18.8).  Otherwise a row of up to 1024 elements is one warp's (four vectors of
+// streamed and from registers: 256 elements 23.6, 17.2; 512: 30.2, 29.5; 1024:
+// 41.4, 46.9; norms with a residual of 256: 40.3, 32.2, of 1024: 79.5, 112; FP32
+// rows of 256: 22.6, 17.9).  Otherwise a row of up to 1024 elements is one warp's (four vectors of
 // 8 a lane), four rows a block; longer rows are a block's, with the fewest
 // vectors a thread that 1024 threads cover; beyond 32768 elements the row is
 // read twice.

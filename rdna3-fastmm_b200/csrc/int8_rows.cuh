@@ -46,7 +46,7 @@ __device__ __forceinline__ void wait_for_previous_kernel() {
 __device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;"); }
 
 constexpr int kRowsMaxThreads = 1024;
-constexpr int kRowsNormThreads = 768;  // streamed norms: 80 registers a thread (65536 x 4608: 349 us with 64, 333)
+constexpr int kRowsNormThreads = 768;  // streamed norms: 80 registers a thread (65536 x 4608: 349 us with 64, 334)
 
 struct Int8RowsParams {
   const void* x;

@@ -321,8 +321,9 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: torch.Tensor 
 
     ``h`` is rounded to ``x``'s type (BF16 or FP16), returned as the new
     residual, and read by the norm; ``y = h * weight / sqrt(mean(h^2) + eps)``
-    is quantised unrounded as by ``quantize_rows``.  ``weight[K]`` has ``x``'s
-    type or FP32.  ``residual_out`` may be ``residual`` or ``x`` itself, which
+    is quantised unrounded as by ``quantize_rows``.  A row has codes 0 and scale
+    NaN where a value, its square or its gain is not finite in FP32, or the
+    scale is beyond FP32.  ``weight[K]`` has ``x``'s type or FP32.  ``residual_out`` may be ``residual`` or ``x`` itself, which
     updates the stream in place."""
     device = _require_cuda(x, "x")
     kind = x.dtype
